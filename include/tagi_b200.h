@@ -502,6 +502,85 @@ int tagi_rmsnorm_backward(const float* dmz, const float* dSz, const float* ma,
 int tagi_apply_vector_sums(const double* g_m, const double* g_S, int64_t n, int mode, float* m,
                            float* S, float* d_m, float* d_S, float cap_factor, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Token path: scaled embedding, residual RMSNorm, 8-bit linear layers
+ * (no reference counterpart beyond embedding.py:88-151 and rms_norm.py:93-137)
+ * ------------------------------------------------------------------------- */
+
+/* Scaled embedding lookup of n tokens: mz[t] = scale*mw[id], Sz[t] =
+ * scale^2*Sw[id]. ids: n values of id_type 0 (float32, truncated toward zero,
+ * V <= 2^24), 1 (int32) or 2 (int64). Ids outside [0, V) and padding_idx give
+ * zero rows. mw, Sw: V x D; mz, Sz: n x D. */
+int tagi_embedding_lookup(const void* ids, int id_type, const float* mw, const float* Sw,
+                          float* mz, float* Sz, int64_t n, int64_t V, int64_t D,
+                          int64_t padding_idx, float scale, void* stream);
+
+/* Its gradient, over tokens sorted by id: g_m[v] = scale * sum of dmz and g_S[v] =
+ * scale^2 * sum of dSz over the tokens of row v (dmz, dSz: n x D). Mode
+ * TAGI_WGRAD_SUMS writes them (V x D, zero rows where no token is),
+ * TAGI_WGRAD_DELTAS writes Sw*g_m and Sw^2*g_S, TAGI_WGRAD_UPDATE applies the
+ * capped update (tagi_capped_update) to the rows of mw, Sw that a token names and
+ * leaves the others as they are. Deterministic. n <= 2^30, D <= 2^20. */
+size_t tagi_embedding_grad_workspace_size(int64_t n, int64_t D);
+int tagi_embedding_grad(const void* ids, int id_type, const float* dmz, const float* dSz,
+                        int64_t n, int64_t V, int64_t D, int64_t padding_idx, float scale,
+                        int mode, float* mw, float* Sw, float* out_m, float* out_S,
+                        float cap_factor, void* workspace, size_t workspace_bytes, void* stream);
+
+/* h = (ma + mr, Sa + Sr) into hm, hS, then tagi_rmsnorm_forward of h. mr, Sr NULL:
+ * no residual (hm, hS are not written). */
+int tagi_add_rmsnorm_forward(const float* ma, const float* Sa, const float* mr, const float* Sr,
+                             const float* mw, const float* Sw, float* hm, float* hS, float* mz,
+                             float* Sz, float* inv_rms, int64_t rows, int64_t ni, float eps,
+                             void* stream);
+
+/* The same with the output in 8 bits: codes of the means (signed), the squared
+ * means and the variances (unsigned), rows ldq bytes apart, and their scales
+ * (3 x rows: means, squares, variances); value = code * scale. A row that holds a
+ * value that is not finite has codes 0 and scales NaN. */
+int tagi_add_rmsnorm_int8(const float* ma, const float* Sa, const float* mr, const float* Sr,
+                          const float* mw, const float* Sw, float* hm, float* hS, int8_t* q_m,
+                          uint8_t* q_2, uint8_t* q_S, float* scales, int64_t ldq, int64_t rows,
+                          int64_t ni, float eps, void* stream);
+
+/* Rows (means m, variances S) put into 8 bits without a norm: q_m of m, q_2 of m^2
+ * (weights != 0: of m^2 + S), q_S of S, scales as above. Negative variances count
+ * as 0. */
+int tagi_quantize_moments(const float* m, const float* S, int weights, int8_t* q_m, uint8_t* q_2,
+                          uint8_t* q_S, float* scales, int64_t ldq, int64_t rows, int64_t ni,
+                          void* stream);
+/* code * scale of all three, rows x ni each. */
+int tagi_int8_values(const int8_t* q_m, const uint8_t* q_2, const uint8_t* q_S,
+                     const float* scales, int64_t ldq, float* v_m, float* v_2, float* v_S,
+                     int64_t rows, int64_t ni, void* stream);
+
+/* Backward of tagi_add_rmsnorm_forward: d_m = rm + inv*mw*dmz, d_S = rS +
+ * (inv*mw)^2*dSz (the deltas of both branches; rm, rS: the deltas that reach the
+ * stream h behind the norm, NULL for none) and the gamma sums over rows, as
+ * tagi_rmsnorm_backward forms them: mode TAGI_WGRAD_SUMS writes sums (2*ni
+ * float64), TAGI_WGRAD_DELTAS d_mw and d_Sw, TAGI_WGRAD_UPDATE applies the capped
+ * update to mw, Sw. */
+size_t tagi_add_rmsnorm_backward_workspace_size(int64_t rows, int64_t ni);
+int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, const float* hm,
+                              const float* inv_rms, const float* rm, const float* rS, float* d_m,
+                              float* d_S, int mode, double* sums, float* mw, float* Sw,
+                              float* d_mw, float* d_Sw, float cap_factor, int64_t rows, int64_t ni,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Mean and variance of a linear layer from 8-bit operands: x (M x K, tokens, from
+ * tagi_add_rmsnorm_int8 or tagi_quantize_moments) and w (N x K, output channels,
+ * from tagi_quantize_moments with weights != 0):
+ *   mz = x_scales[0] w_scales[0] (x_m w_m^T) + mb
+ *   Sz = x_scales[1] w_scales[2] (x_2 w_S^T) + x_scales[2] w_scales[1] (x_S w_2^T) + Sb
+ * with exact 32-bit integer sums; mz, Sz: M x N float32; mb, Sb: N floats or NULL.
+ * Rows of codes start on 16-byte boundaries (pointers and ldx, ldw multiples of
+ * 16); 1 <= K <= 33025. */
+int tagi_int8_moment_matmul(const int8_t* x_m, const uint8_t* x_2, const uint8_t* x_S,
+                            const float* x_scales, int64_t ldx, const int8_t* w_m,
+                            const uint8_t* w_2, const uint8_t* w_S, const float* w_scales,
+                            int64_t ldw, const float* mb, const float* Sb, float* mz, float* Sz,
+                            int64_t M, int64_t N, int64_t K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -49,6 +49,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "int8_linear.cuh"
 #include "moment_gemm.cuh"
 
 namespace tagi {
@@ -1581,6 +1582,8 @@ int launch_bn(const GemmArgs& g, int bn, int batch, cudaStream_t st, const char*
 
 }  // namespace
 
+void count_tc_launch() { ++g_tc_launches; }
+
 int tc_pick(int vm, int M, int N, int Kr, int batch, bool fill) {
     (void)vm;
     if (!tc_enabled()) return 0;
@@ -1717,6 +1720,7 @@ extern "C" int tagi_set_wait_limit_ns(uint64_t ns) {
     const int force = (ns > 0 && ns < 1000) ? 1 : 0;
     cudaError_t e = cudaMemcpyToSymbol(tagi::g_wait_limit_ns, &v, sizeof(v));
     if (e == cudaSuccess) e = cudaMemcpyToSymbol(tagi::g_force_abort, &force, sizeof(force));
+    if (e == cudaSuccess) e = tagi::int8_set_wait_limit(v, force);
     if (e != cudaSuccess) {
         cudaGetLastError();
         tagi::set_error("tagi_set_wait_limit_ns: %s", cudaGetErrorString(e));
@@ -1737,5 +1741,6 @@ extern "C" int tagi_device_status(int reset) {
         const int zero = 0;
         cudaMemcpyToSymbol(tagi::g_device_error, &zero, sizeof(int));
     }
-    return v;
+    const int v8 = tagi::int8_device_status(reset);
+    return v != 0 ? v : v8;
 }

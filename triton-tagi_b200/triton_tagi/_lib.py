@@ -68,6 +68,16 @@ _SIGS = {
     "tagi_rmsnorm_forward": "ppppppp" + "ii" + "f" + "p",
     "tagi_rmsnorm_backward": "pppppppp" + "ii" + "p",
     "tagi_apply_vector_sums": "pp" + "i" + "n" + "pppp" + "f" + "p",
+    "tagi_embedding_lookup": "pn" + "pppp" + "iiii" + "f" + "p",
+    "tagi_embedding_grad_workspace_size": "ii",
+    "tagi_embedding_grad": "pn" + "pp" + "iiii" + "f" + "n" + "pppp" + "f" + "pz" + "p",
+    "tagi_add_rmsnorm_forward": "p" * 11 + "ii" + "f" + "p",
+    "tagi_add_rmsnorm_int8": "p" * 12 + "iii" + "f" + "p",
+    "tagi_quantize_moments": "ppn" + "pppp" + "iii" + "p",
+    "tagi_int8_values": "pppp" + "i" + "ppp" + "ii" + "p",
+    "tagi_add_rmsnorm_backward_workspace_size": "ii",
+    "tagi_add_rmsnorm_backward": "p" * 8 + "n" + "ppppp" + "f" + "ii" + "pz" + "p",
+    "tagi_int8_moment_matmul": "ppppi" + "ppppi" + "pppp" + "iii" + "p",
     "tagi_version": "",
     "tagi_device_arch": "n",
     "tagi_last_error": "",
@@ -88,6 +98,8 @@ _RET = {
     "tagi_fused_weight_grad_workspace_size": _Z,
     "tagi_param_grad_workspace_size": _Z,
     "tagi_store_workspace_size": _Z,
+    "tagi_embedding_grad_workspace_size": _Z,
+    "tagi_add_rmsnorm_backward_workspace_size": _Z,
     "tagi_last_error": ctypes.c_char_p,
     "tagi_kernel_launches": ctypes.c_uint64,
     "tagi_tma_launches": ctypes.c_uint64,
@@ -194,6 +206,28 @@ def check_cuda_f32(*ts: torch.Tensor) -> None:
             raise ValueError("triton_tagi (B200) tensors must live on a CUDA device")
         if t.dtype != torch.float32:
             raise ValueError(f"expected float32 tensor, got {t.dtype}")
+
+
+def check_same_device(*ts: torch.Tensor | None) -> None:
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors live on different devices ({dev} and {t.device})")
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``lib()(name, *args, stream)`` with ``t``'s device current and its current
+    stream: a kernel belongs to the device that is current when it is launched."""
+    dev = t.device
+    if dev.index == torch.cuda.current_device():
+        lib()(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            lib()(name, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 def workspace(nbytes: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int | None, int]:
