@@ -419,14 +419,31 @@ int launch_norm(const NormArgs& g, cudaStream_t st, const char* what) {
     return launch_width<OUT, 1>(g, st, what);
 }
 
+// code * scale, VEC codes of one of the three operands (blockIdx.y) per thread.
+template <int VEC>
 __global__ void values_kernel(const NormArgs g, float* vm, float* v2, float* vS) {
-    const int64_t total = g.rows * g.ni;
+    const int which = blockIdx.y;
+    const int per = g.ni / VEC;
+    const int64_t total = g.rows * per;
+    const uint8_t* q = which == 0 ? reinterpret_cast<const uint8_t*>(g.qm)
+                                  : (which == 1 ? g.q2 : g.qS);
+    float* v = which == 0 ? vm : (which == 1 ? v2 : vS);
+    const float* sc = g.scales + which * g.rows;
     for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t r = i / g.ni, o = r * g.ldq + (i - r * g.ni);
-        vm[i] = static_cast<float>(g.qm[o]) * g.scales[r];
-        v2[i] = static_cast<float>(g.q2[o]) * g.scales[g.rows + r];
-        vS[i] = static_cast<float>(g.qS[o]) * g.scales[2 * g.rows + r];
+        const int64_t r = i / per;
+        const int j = static_cast<int>(i - r * per) * VEC;
+        const float s = sc[r];
+        const uint8_t* p = q + r * g.ldq + j;
+        uint32_t x = VEC == 4 ? *reinterpret_cast<const uint32_t*>(p) : *p;
+        float out[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const uint32_t b = (x >> (8 * e)) & 255u;
+            out[e] = s * (which == 0 ? static_cast<float>(static_cast<int8_t>(b))
+                                     : static_cast<float>(b));
+        }
+        st<VEC>(v + r * g.ni + j, out);
     }
 }
 
@@ -498,30 +515,36 @@ __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackArgs g) {
     }
 }
 
-// Adds the slices' sums of 32 columns: 8 threads per column, each every 8th slice.
+// Adds the slices' sums: 8 columns per block, 32 threads per column, each every 32nd
+// slice (a fixed order), their sums by a shuffle tree of fixed shape.
 __global__ void __launch_bounds__(256) back_finish_kernel(const double* part, int slices, int ni,
                                                           int mode, double* sums, float* w,
                                                           float* Sw, float* d_w, float* d_Sw,
                                                           float cap) {
-    __shared__ double red[2][8][32];
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int j = blockIdx.x * 32 + lane;
+    __shared__ double red[2][8][33];
+    const int c = threadIdx.x & 7, g = threadIdx.x >> 3;
+    const int col = blockIdx.x * 8 + c;
     double a = 0.0, b = 0.0;
-    if (j < ni) {
-#pragma unroll 4
-        for (int s = g; s < slices; s += 8) {
-            a += part[static_cast<int64_t>(s) * 2 * ni + j];
-            b += part[static_cast<int64_t>(s) * 2 * ni + ni + j];
+    if (col < ni) {
+#pragma unroll 8
+        for (int s = g; s < slices; s += 32) {
+            a += part[static_cast<int64_t>(s) * 2 * ni + col];
+            b += part[static_cast<int64_t>(s) * 2 * ni + ni + col];
         }
     }
-    red[0][g][lane] = a;
-    red[1][g][lane] = b;
+    red[0][c][g] = a;
+    red[1][c][g] = b;
     __syncthreads();
-    if (g != 0 || j >= ni) return;
-    for (int k = 1; k < 8; ++k) {
-        a += red[0][k][lane];
-        b += red[1][k][lane];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;  // a warp per column
+    a = red[0][warp][lane];
+    b = red[1][warp][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
     }
+    const int j = blockIdx.x * 8 + warp;
+    if (lane != 0 || j >= ni) return;
     if (mode == TAGI_WGRAD_SUMS) {
         sums[j] = a;
         sums[ni + j] = b;
@@ -543,7 +566,7 @@ __global__ void __launch_bounds__(256) back_finish_kernel(const double* part, in
 // Slices of rows: enough blocks to fill the SMs several times, 8 rows or more each.
 int slices_of(int64_t rows, int64_t ni) {
     const int64_t cols = (ni + 4 * kBackThreads - 1) / (4 * kBackThreads);
-    int64_t s = (kNumSMs * 8 + cols - 1) / cols;
+    int64_t s = (kNumSMs * 4 + cols - 1) / cols;
     const int64_t most = (rows + 7) / 8;
     if (s > most) s = most;
     return static_cast<int>(s < 1 ? 1 : s);
@@ -626,7 +649,20 @@ extern "C" int tagi_int8_values(const int8_t* q_m, const uint8_t* q_2, const uin
     g.qm = const_cast<int8_t*>(q_m); g.q2 = const_cast<uint8_t*>(q_2);
     g.qS = const_cast<uint8_t*>(q_S); g.scales = const_cast<float*>(scales);
     g.ldq = ldq; g.rows = rows; g.ni = static_cast<int>(ni);
-    values_kernel<<<grid_1d(rows * ni, 256), 256, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
+    uintptr_t bits = static_cast<uintptr_t>(ldq) * 4;  // codes on 4 bytes, values on 16
+    for (const void* p : {static_cast<const void*>(v_m), static_cast<const void*>(v_2),
+                          static_cast<const void*>(v_S)})
+        bits |= reinterpret_cast<uintptr_t>(p);
+    for (const void* p : {static_cast<const void*>(q_m), static_cast<const void*>(q_2),
+                          static_cast<const void*>(q_S)})
+        bits |= reinterpret_cast<uintptr_t>(p) * 4;
+    if (ni % 4 == 0 && (bits & 15) == 0) {
+        const dim3 grid(grid_1d(rows * (ni / 4), 256), 3);
+        values_kernel<4><<<grid, 256, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
+    } else {
+        const dim3 grid(grid_1d(rows * ni, 256), 3);
+        values_kernel<1><<<grid, 256, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
+    }
     return check_launch(what);
 }
 
@@ -681,7 +717,7 @@ extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, con
         back_kernel<1><<<grid, kBackThreads, 0, st>>>(g);
     const int rc = check_launch(what);
     if (rc) return rc;
-    back_finish_kernel<<<static_cast<unsigned>((ni + 31) / 32), 256, 0, st>>>(
+    back_finish_kernel<<<static_cast<unsigned>((ni + 7) / 8), 256, 0, st>>>(
         g.part, slices, g.ni, mode, sums, mw, Sw, d_mw, d_Sw, cap_factor);
     return check_launch(what);
 }

@@ -208,26 +208,42 @@ def check_cuda_f32(*ts: torch.Tensor) -> None:
             raise ValueError(f"expected float32 tensor, got {t.dtype}")
 
 
-def check_same_device(*ts: torch.Tensor | None) -> None:
-    dev = None
+def check_f32(*ts: torch.Tensor | None) -> int:
+    """Checks that the tensors (None: absent) are float32 on one CUDA device and
+    returns its index."""
+    dev = -1
     for t in ts:
         if t is None:
             continue
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors live on different devices ({dev} and {t.device})")
+        if t.dtype is not torch.float32:
+            raise ValueError(f"expected float32 tensor, got {t.dtype}")
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
+                raise ValueError("triton_tagi (B200) tensors must live on a CUDA device")
+            if dev >= 0:
+                raise ValueError(f"tensors live on different devices (cuda:{dev} and cuda:{d})")
+            dev = d
+    return dev
 
 
-def call_on(t: torch.Tensor, name: str, *args) -> None:
-    """``lib()(name, *args, stream)`` with ``t``'s device current and its current
+def check_on(dev: int, *ts: torch.Tensor | None) -> None:
+    """Checks that the tensors live on CUDA device ``dev``."""
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors live on different devices (cuda:{dev} and {t.device})"
+                             if t.is_cuda else
+                             "triton_tagi (B200) tensors must live on a CUDA device")
+
+
+def call_on(dev: int, name: str, *args) -> None:
+    """``lib()(name, *args, stream)`` with device ``dev`` current and its current
     stream: a kernel belongs to the device that is current when it is launched."""
-    dev = t.device
-    if dev.index == torch.cuda.current_device():
-        lib()(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    if dev == torch._C._cuda_getDevice():
+        lib()(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            lib()(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            lib()(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def workspace(nbytes: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int | None, int]:

@@ -18,15 +18,13 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_cuda_f32,
-                    check_same_device, lib, ptr, workspace)
+from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on, lib,
+                    ptr, workspace)
 
 _ID_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
 
-def _check_ids(ids: Tensor) -> int:
-    if not ids.is_cuda:
-        raise ValueError("triton_tagi (B200) tensors must live on a CUDA device")
+def _id_type(ids: Tensor) -> int:
     code = _ID_TYPES.get(ids.dtype)
     if code is None:
         raise ValueError(f"token ids must be int64, int32 or float32, got {ids.dtype}")
@@ -41,30 +39,30 @@ def _check_table(mw: Tensor, Sw: Tensor) -> None:
 def embedding_lookup(ids: Tensor, mw: Tensor, Sw: Tensor, scale: float = 1.0,
                      padding_idx: int = -1) -> tuple[Tensor, Tensor]:
     """(mz, Sz), each ``(*ids.shape, D)``: rows s·mw[id] and s²·Sw[id]."""
-    code = _check_ids(ids)
-    check_cuda_f32(mw, Sw)
-    check_same_device(ids, mw, Sw)
+    code = _id_type(ids)
+    dev = check_f32(mw, Sw)
+    check_on(dev, ids)
     _check_table(mw, Sw)
     ids, mw, Sw = ids.contiguous(), mw.contiguous(), Sw.contiguous()
     V, D = mw.shape
-    mz = torch.empty((*ids.shape, D), device=mw.device)
+    mz = mw.new_empty((*ids.shape, D))
     Sz = torch.empty_like(mz)
-    call_on(mw, "tagi_embedding_lookup", ids.data_ptr(), code, mw.data_ptr(), Sw.data_ptr(),
+    call_on(dev, "tagi_embedding_lookup", ids.data_ptr(), code, mw.data_ptr(), Sw.data_ptr(),
             mz.data_ptr(), Sz.data_ptr(), ids.numel(), V, D, padding_idx, scale)
     return mz, Sz
 
 
 def _grad(mode, ids, dmz, dSz, V, D, scale, padding_idx, mw, Sw, out_m, out_S, cap) -> None:
-    code = _check_ids(ids)
-    check_cuda_f32(dmz, dSz)
-    check_same_device(ids, dmz, dSz, mw, Sw, out_m, out_S)
+    code = _id_type(ids)
+    dev = check_f32(dmz, dSz, mw, Sw, out_m, out_S)
+    check_on(dev, ids)
     n = ids.numel()
     if dmz.shape != dSz.shape or dmz.numel() != n * D or (dmz.dim() and dmz.shape[-1] != D):
         raise ValueError(f"deltas {tuple(dmz.shape)} and {tuple(dSz.shape)} do not match "
                          f"{n} tokens of {D} columns")
     ids, dmz, dSz = ids.contiguous(), dmz.contiguous(), dSz.contiguous()
     hold, wp, wn = workspace(lib().size("tagi_embedding_grad_workspace_size", n, D), dmz)
-    call_on(dmz, "tagi_embedding_grad", ids.data_ptr(), code, dmz.data_ptr(), dSz.data_ptr(), n,
+    call_on(dev, "tagi_embedding_grad", ids.data_ptr(), code, dmz.data_ptr(), dSz.data_ptr(), n,
             V, D, padding_idx, scale, mode, ptr(mw), ptr(Sw), ptr(out_m), ptr(out_S), cap, wp, wn)
 
 
@@ -78,16 +76,14 @@ def embedding_grad(ids: Tensor, dmz: Tensor, dSz: Tensor, num_embeddings: int, s
     if num_embeddings < 1 or D < 1:
         raise ValueError("embedding_grad: an empty table")
     if Sw is not None:
-        check_cuda_f32(Sw)
         if tuple(Sw.shape) != (num_embeddings, D):
             raise ValueError(f"Sw {tuple(Sw.shape)} is not ({num_embeddings}, {D})")
         Sw = Sw.contiguous()
     if out is None:
-        g_m = torch.empty(num_embeddings, D, device=dmz.device)
+        g_m = dmz.new_empty((num_embeddings, D))
         g_S = torch.empty_like(g_m)
     else:
         g_m, g_S = out
-        check_cuda_f32(g_m, g_S)
         for t in out:
             if tuple(t.shape) != (num_embeddings, D) or not t.is_contiguous():
                 raise ValueError(f"out must be contiguous ({num_embeddings}, {D}) tensors")
@@ -101,7 +97,6 @@ def embedding_update(ids: Tensor, dmz: Tensor, dSz: Tensor, mw: Tensor, Sw: Tens
     """The capped update of (mw, Sw) from the deltas, in place, as ``update_parameters``
     with ``embedding_grad(..., Sw=Sw)`` would apply it to the rows that a token names;
     the other rows are neither read nor written."""
-    check_cuda_f32(mw, Sw)
     _check_table(mw, Sw)
     if not (mw.is_contiguous() and Sw.is_contiguous()):
         raise ValueError("in-place targets must be contiguous")

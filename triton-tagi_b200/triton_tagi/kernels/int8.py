@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 from torch import Tensor
 
-from .._lib import call_on, check_cuda_f32, check_same_device, ptr
+from .._lib import call_on, check_f32, check_on, ptr
 
 
 class Int8Moments(NamedTuple):
@@ -36,21 +36,24 @@ class Int8Moments(NamedTuple):
 
     def values(self) -> tuple[Tensor, Tensor, Tensor]:
         """What the codes stand for: three float32 ``(rows, width)`` tensors."""
-        q = _checked(self)
+        dev = check_f32(self.scales)
+        q = _checked(self, dev)
         rows, width = q.q_m.shape
-        out = [torch.empty(rows, width, device=q.scales.device) for _ in range(3)]
-        call_on(q.scales, "tagi_int8_values", *_pointers(q), *(t.data_ptr() for t in out), rows,
+        out = [q.scales.new_empty((rows, width)) for _ in range(3)]
+        call_on(dev, "tagi_int8_values", *_pointers(q), *(t.data_ptr() for t in out), rows,
                 width)
         return tuple(out)
 
 
-def empty_codes(rows: int, width: int, device) -> Int8Moments:
+def empty_codes(rows: int, width: int, like: Tensor) -> Int8Moments:
     """Uninitialised codes whose rows start on 16-byte boundaries, as the tensor-core
     product's copies need them."""
     ld = (width + 15) // 16 * 16
-    q = [torch.empty_strided((rows, width), (ld, 1), dtype=t, device=device)
-         for t in (torch.int8, torch.uint8, torch.uint8)]
-    return Int8Moments(*q, torch.empty(3, rows, device=device))
+    new = like.new_empty_strided
+    size, stride = (rows, width), (ld, 1)
+    return Int8Moments(new(size, stride, dtype=torch.int8), new(size, stride, dtype=torch.uint8),
+                       new(size, stride, dtype=torch.uint8),
+                       like.new_empty((3, rows), dtype=torch.float32))
 
 
 def _ld(t: Tensor) -> int:
@@ -58,12 +61,11 @@ def _ld(t: Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
-def _checked(q: Int8Moments) -> Int8Moments:
+def _checked(q: Int8Moments, dev: int) -> Int8Moments:
     """``q`` with the layout the kernels read: unit column stride, one row stride, rows
     on 16-byte boundaries (copied where it differs)."""
     q_m, q_2, q_S, scales = q
-    check_cuda_f32(scales)
-    check_same_device(q_m, q_2, q_S, scales)
+    check_on(dev, q_m, q_2, q_S)
     if q_m.dtype != torch.int8 or q_2.dtype != torch.uint8 or q_S.dtype != torch.uint8:
         raise ValueError(f"codes must be int8, uint8, uint8, got {q_m.dtype}, {q_2.dtype}, "
                          f"{q_S.dtype}")
@@ -74,7 +76,7 @@ def _checked(q: Int8Moments) -> Int8Moments:
     ld = _ld(q_m)
     if any(t.stride(1) != 1 or _ld(t) != ld or ld < t.shape[1] or (ld | t.data_ptr()) & 15
            for t in (q_m, q_2, q_S)):
-        new = empty_codes(*q_m.shape, q_m.device)
+        new = empty_codes(*q_m.shape, scales)
         for a, b in zip(new[:3], (q_m, q_2, q_S)):
             a.copy_(b)
         q = Int8Moments(*new[:3], scales)
@@ -86,15 +88,14 @@ def _pointers(q: Int8Moments) -> tuple:
 
 
 def _quantize(m: Tensor, S: Tensor, weights: bool) -> Int8Moments:
-    check_cuda_f32(m, S)
-    check_same_device(m, S)
+    dev = check_f32(m, S)
     if m.dim() < 1 or m.shape != S.shape or m.shape[-1] < 1:
         raise ValueError(f"means {tuple(m.shape)} and variances {tuple(S.shape)} must have one "
                          "shape and a last dimension")
     width = m.shape[-1]
     m, S = m.reshape(-1, width).contiguous(), S.reshape(-1, width).contiguous()
-    q = empty_codes(m.shape[0], width, m.device)
-    call_on(m, "tagi_quantize_moments", m.data_ptr(), S.data_ptr(), 1 if weights else 0,
+    q = empty_codes(m.shape[0], width, m)
+    call_on(dev, "tagi_quantize_moments", m.data_ptr(), S.data_ptr(), 1 if weights else 0,
             *_pointers(q), m.shape[0], width)
     return q
 
@@ -116,9 +117,8 @@ def int8_moments_matmul(x: Int8Moments, w: Int8Moments, mb: Tensor | None = None
                         Sb: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """(mz, Sz), each ``(M, N)``: the moments of tokens ``x`` (M, K) through weights
     ``w`` (N, K) plus the biases (N values each, or None)."""
-    x, w = _checked(x), _checked(w)
-    check_cuda_f32(mb, Sb)
-    check_same_device(x.scales, w.scales, mb, Sb)
+    dev = check_f32(x.scales, w.scales, mb, Sb)
+    x, w = _checked(x, dev), _checked(w, dev)
     M, K = x.q_m.shape
     N = w.q_m.shape[0]
     if w.q_m.shape[1] != K:
@@ -127,8 +127,8 @@ def int8_moments_matmul(x: Int8Moments, w: Int8Moments, mb: Tensor | None = None
         raise ValueError(f"biases must hold {N} values")
     mb = None if mb is None else mb.contiguous()
     Sb = None if Sb is None else Sb.contiguous()
-    mz = torch.empty(M, N, device=x.scales.device)
+    mz = x.scales.new_empty((M, N))
     Sz = torch.empty_like(mz)
-    call_on(mz, "tagi_int8_moment_matmul", *_pointers(x), *_pointers(w), ptr(mb), ptr(Sb),
+    call_on(dev, "tagi_int8_moment_matmul", *_pointers(x), *_pointers(w), ptr(mb), ptr(Sb),
             mz.data_ptr(), Sz.data_ptr(), M, N, K)
     return mz, Sz

@@ -12,25 +12,24 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_cuda_f32,
-                    check_same_device, lib, ptr, workspace)
+from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on, lib,
+                    ptr, workspace)
 from .int8 import Int8Moments, _pointers, empty_codes
 
 
-def _rows(name: str, mw: Tensor, Sw: Tensor | None, *ts: Tensor | None) -> tuple[int, int]:
-    """(rows, width) of the tensors given (None: absent), after checking them."""
-    check_cuda_f32(mw, Sw, *ts)
-    check_same_device(mw, Sw, *ts)
-    first = next(t for t in ts if t is not None)
+def _rows(name: str, mw: Tensor, Sw: Tensor | None, *ts: Tensor | None) -> tuple[int, int, int]:
+    """(device, rows, width) of the tensors given (None: absent), after checking them."""
+    dev = check_f32(mw, Sw, *ts)
+    first = ts[0]
     width = mw.numel()
     if width < 1 or Sw is not None and Sw.numel() != width:
         raise ValueError(f"{name}: scale parameters of {mw.numel()} and "
                          f"{'no' if Sw is None else Sw.numel()} values")
     for t in ts:
-        if t is not None and (t.shape != first.shape or t.dim() < 1 or t.shape[-1] != width):
+        if t is not None and (t.dim() < 1 or t.shape[-1] != width or t.shape != first.shape):
             raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit {tuple(first.shape)} "
                              f"with rows of {width}")
-    return first.numel() // width, width
+    return dev, first.numel() // width, width
 
 
 def _pair(name: str, a: Tensor | None, b: Tensor | None) -> None:
@@ -47,12 +46,12 @@ def add_rmsnorm(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | None, mw
     """(μ_h, S_h, μ_z, S_z, inv): the stream, its norm and the rows' 1/rms. Without a
     residual (mr, Sr None) the stream is the input itself."""
     _pair("add_rmsnorm", mr, Sr)
-    rows, width = _rows("add_rmsnorm", mw, Sw, ma, Sa, mr, Sr)
+    dev, rows, width = _rows("add_rmsnorm", mw, Sw, ma, Sa, mr, Sr)
     ma, Sa, mr, Sr, mw, Sw = _cont(ma, Sa, mr, Sr, mw, Sw)
     hm, hS = (ma, Sa) if mr is None else (torch.empty_like(ma), torch.empty_like(Sa))
     mz, Sz = torch.empty_like(ma), torch.empty_like(Sa)
-    inv = torch.empty(ma.shape[:-1], device=ma.device)
-    call_on(ma, "tagi_add_rmsnorm_forward", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
+    inv = ma.new_empty(ma.shape[:-1])
+    call_on(dev, "tagi_add_rmsnorm_forward", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
             mw.data_ptr(), Sw.data_ptr(), hm.data_ptr(), hS.data_ptr(), mz.data_ptr(),
             Sz.data_ptr(), inv.data_ptr(), rows, width, eps)
     return hm, hS, mz, Sz, inv
@@ -63,11 +62,11 @@ def add_rmsnorm_int8(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | Non
     """(μ_h, S_h, codes): as ``add_rmsnorm`` with the norm's output in 8 bits, leading
     dimensions flattened to rows. The codes do not depend on how a row was summed."""
     _pair("add_rmsnorm_int8", mr, Sr)
-    rows, width = _rows("add_rmsnorm_int8", mw, Sw, ma, Sa, mr, Sr)
+    dev, rows, width = _rows("add_rmsnorm_int8", mw, Sw, ma, Sa, mr, Sr)
     ma, Sa, mr, Sr, mw, Sw = _cont(ma, Sa, mr, Sr, mw, Sw)
     hm, hS = (ma, Sa) if mr is None else (torch.empty_like(ma), torch.empty_like(Sa))
-    q = empty_codes(rows, width, ma.device)
-    call_on(ma, "tagi_add_rmsnorm_int8", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
+    q = empty_codes(rows, width, ma)
+    call_on(dev, "tagi_add_rmsnorm_int8", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
             mw.data_ptr(), Sw.data_ptr(), hm.data_ptr(), hS.data_ptr(), *_pointers(q), rows,
             width, eps)
     return hm, hS, q
@@ -76,9 +75,8 @@ def add_rmsnorm_int8(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | Non
 def _backward(mode, dmz, dSz, hm, inv, mw, Sw, rm, rS, sums=None, d_mw=None, d_Sw=None, cap=1.0):
     name = "add_rmsnorm_backward"
     _pair(name, rm, rS)
-    rows, width = _rows(name, mw, Sw, dmz, dSz, rm, rS)
-    check_cuda_f32(hm, inv)
-    check_same_device(dmz, hm, inv)
+    dev, rows, width = _rows(name, mw, Sw, dmz, dSz, rm, rS)
+    check_f32(dmz, hm, inv)
     if hm.numel() != rows * width or inv.numel() != rows:
         raise ValueError(f"{name}: the stream {tuple(hm.shape)} and 1/rms {tuple(inv.shape)} do "
                          f"not match {rows} rows of {width}")
@@ -86,7 +84,7 @@ def _backward(mode, dmz, dSz, hm, inv, mw, Sw, rm, rS, sums=None, d_mw=None, d_S
     d_m, d_S = torch.empty_like(dmz), torch.empty_like(dSz)
     hold, wp, wn = workspace(lib().size("tagi_add_rmsnorm_backward_workspace_size", rows, width),
                              dmz)
-    call_on(dmz, "tagi_add_rmsnorm_backward", dmz.data_ptr(), dSz.data_ptr(), hm.data_ptr(),
+    call_on(dev, "tagi_add_rmsnorm_backward", dmz.data_ptr(), dSz.data_ptr(), hm.data_ptr(),
             inv.data_ptr(), ptr(rm), ptr(rS), d_m.data_ptr(), d_S.data_ptr(), mode, ptr(sums),
             mw.data_ptr(), ptr(Sw), ptr(d_mw), ptr(d_Sw), cap, rows, width, wp, wn)
     return d_m, d_S
@@ -109,7 +107,7 @@ def add_rmsnorm_backward_sums(dmz, dSz, hm, inv, mw, sums, rm=None, rS=None) -> 
     ``sums`` (2 × width float64, contiguous), for a data-parallel reduction."""
     if sums.dtype != torch.float64 or sums.numel() != 2 * mw.numel() or not sums.is_contiguous():
         raise ValueError("sums must hold 2 x width contiguous float64 values")
-    check_same_device(dmz, sums)
+    check_on(dmz.get_device(), sums)
     return _backward(WGRAD_SUMS, dmz, dSz, hm, inv, mw.contiguous(), None, rm, rS, sums=sums)
 
 
