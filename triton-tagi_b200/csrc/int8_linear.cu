@@ -8,20 +8,32 @@
 // w: codes of the weights' means, mu^2 + S and variances; a, b: the scales of each
 // token and of each output channel. The three products are exact (32-bit sums).
 //
-// Tiles. The weights are the A operand (128 channels: tensor-memory lanes) and the
-// tokens the B operand (BN columns), so a lane is a channel: its scales and bias are
-// registers, and for one token a warp stores 32 neighbouring channels of a row of the
-// output straight from tensor memory. Few tokens take a narrow B tile (16 columns)
-// instead of padding 128 rows. Blocks of grid.z 0 form the variance (two products,
-// two accumulators), those of grid.z 1 the mean.
+// The weights are the A operand (tensor-memory lanes are channels) and the tokens the
+// B operand (columns), so a lane keeps its channel's scales and bias in registers, and
+// for one token a warp stores 32 neighbouring channels of a row of the output straight
+// from tensor memory. Two kernels:
+//
+// pair_kernel, for many tokens. A cluster of two CTAs computes 256 channels x 256
+// tokens with 2-SM MMAs: each CTA stages its 128 channels and half of the tokens, 64
+// bytes per clock of the tensor pipe's peak and SM, which the L2 delivers (a single-CTA
+// 128 x 128 tile needs 128 and ran at half the rate). Persistent, one pair per two SMs.
+// The three products of a tile follow one another through two accumulators of 256
+// columns: the epilogue warps read one while the MMAs fill the other. The first product
+// of the variance waits in their registers for the second.
+//
+// split_kernel, for few tokens or few tiles. 128 channels x BN tokens (BN from 16);
+// the (product, reduction block) list of a tile is shared out over a cluster of up to
+// 8 CTAs, which exchange their integer sums through distributed shared memory (exact in
+// any order). Bound by the weights' bytes, or by latency.
 //
 // Warp roles: warp 0 issues the tensor-map copies (128 bytes of the reduction of both
-// operands per stage, 128-byte swizzle), warp 1 allocates tensor memory and issues
-// the MMAs, warps 2-5 read the accumulators (lane quarter w % 4) and store.
+// operands per stage, 128-byte swizzle), warp 1 allocates tensor memory and issues the
+// MMAs (in the second CTA of a pair it tells the first which stages have landed), the
+// others read the accumulators (lane quarter w % 4) and store.
 //
-// Every wait is bounded: on timeout a block records an error word
-// (tagi_device_status), stops issuing, lets its own copies and MMAs land and frees
-// its tensor memory.
+// Every wait is bounded: on timeout a CTA records an error word (tagi_device_status),
+// tells its peer, stops issuing, lets its own copies and MMAs land and frees its tensor
+// memory.
 #include <cuda.h>
 
 #include <mutex>
@@ -40,15 +52,6 @@ namespace {
 
 constexpr unsigned long long kDrainNs = 2000000000ull;
 constexpr int kBK = 128;     // bytes of the reduction per stage
-constexpr int kThreads = 192;
-
-template <int BN>
-struct Plan {
-    static constexpr int STAGE = 128 * kBK + BN * kBK;
-    static constexpr int STAGES = BN >= 128 ? 3 : (BN >= 64 ? 4 : 5);
-    static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;
-    static constexpr int SMEM = STAGES * STAGE + 1024;  // 1024: alignment of the swizzled tiles
-};
 
 struct Maps {
     CUtensorMap x[3], w[3];  // means, second operand, variances
@@ -86,24 +89,30 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// False if the block gave up, or if this wait ran out (the block then gives up).
-__device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort,
+struct Abort {
+    volatile int* flag;  // this CTA's abort word
+    uint32_t peer;       // cluster address of the peer CTA's (0: none)
+};
+// False if the CTA gave up, or if this wait ran out (it and its peer then give up).
+__device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, const Abort& ab,
                                             int code) {
     const unsigned long long t0 = globaltimer();
     const unsigned long long limit = *const_cast<volatile unsigned long long*>(&g_int8_wait_ns);
     for (;;) {
         if (mbar_try(bar, parity)) return true;
-        if (*abort) return false;
+        if (*ab.flag) return false;
         if (globaltimer() - t0 > limit) {
-            *abort = 1;
+            *ab.flag = 1;
+            if (ab.peer)
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ab.peer), "r"(1) : "memory");
             atomicCAS(&g_int8_error, 0, code);
             return false;
         }
     }
 }
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const Abort& ab,
                                           int code) {
-    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, abort, code);
+    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, ab, code);
 }
 // For copies and MMAs in flight, which must land before the block may exit.
 __device__ __noinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
@@ -117,6 +126,34 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
                  "r"(bytes)
                  : "memory");
 }
+// Arrive on a barrier given by its cluster address (own or peer CTA), with the default
+// semantics: what these arrivals order are tensor-map copies and tensor-memory reads,
+// which complete before them. (At cluster scope an arrival waits for the warp's output
+// stores and every wait reloads the L1: 8192 x 4096 x 4096 took 548 us instead of 299.)
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr)
+                 : "memory");
+}
+// Address of the same shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_to(uint32_t local, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::
+                     : "memory");
+}
+__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
 // Tile copy from this GPU's own memory to this block alone. x is a multiple of kBK
 // bytes, so it starts on a 16-byte boundary.
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y,
@@ -127,24 +164,47 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
         : "memory");
 }
+// Asynchronous copy of one word to shared memory, or a 0 without reading.
+__device__ __forceinline__ void copy4(float* dst, const float* src, bool read) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(read ? 4 : 0)
+                 : "memory");
+}
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
 __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
+// Arrives on `bar` once all MMAs that this thread issued have completed.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile(
         "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
             smem_u32(bar))
+        : "memory");
+}
+// The same for the pair's MMAs, on the barrier of both CTAs.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"(static_cast<unsigned short>(3))
         : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -154,6 +214,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
           "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait_ld() {
@@ -169,29 +236,279 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
            (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // Instruction descriptor: 32-bit integer accumulator, A and B signed or unsigned
-// 8-bit, M = 128, N = bn.
-__device__ __forceinline__ uint32_t instr_desc(bool sign, int bn) {
+// 8-bit, M = m, N = bn.
+__device__ __forceinline__ uint32_t instr_desc(bool sign, int m, int bn) {
     const uint32_t t = sign ? 1u : 0u;
     return (2u << 4) | (t << 7) | (t << 10) | (static_cast<uint32_t>(bn >> 3) << 17) |
-           (static_cast<uint32_t>(128 >> 4) << 24);
+           (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Products in their order: variance x_2 w_S, variance x_S w_2, mean x_m w_m; the index
+// of the operands and scales (0 means, 1 second operand, 2 variances).
+__device__ __forceinline__ int x_of(int product) { return product == 0 ? 1 : (product == 1 ? 2 : 0); }
+__device__ __forceinline__ int w_of(int product) { return product == 0 ? 2 : (product == 1 ? 1 : 0); }
+
+// ---- many tokens: CTA pairs, persistent ---------------------------------------------
+constexpr int kPairStages = 6;
+constexpr int kPairStage = 2 * 128 * kBK;  // 128 channels and 128 tokens per CTA
+constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+constexpr int kPairReaders = 16;  // epilogue warps: 4 per lane quarter, 64 columns each
+constexpr int kPairThreads = 64 + 32 * kPairReaders;
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    int8_pair_kernel(const Int8Args g, const __grid_constant__ Maps maps) {
+    extern __shared__ char raw[];
+    __shared__ __align__(8) uint64_t landed[kPairStages], peer_landed[kPairStages],
+        empty[kPairStages], acc_full[2], acc_empty[2], done;
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag;
+    __shared__ __align__(16) float scale[2][3][256];  // the tile's tokens, by product
+    __shared__ float chan[2][5][128];                 // this CTA's channels: by product, Sb, mb
+    char* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int kblocks = (g.K + kBK - 1) / kBK;
+    const int ctiles = (g.N + 255) / 256;
+    const int tiles = ctiles * ((g.M + 255) / 256);
+    const int pairs = gridDim.x / 2;
+    const Abort ab{&abort_flag, map_to(smem_u32(&abort_flag), rank ^ 1)};
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            mbar_init(&landed[s], 1);
+            mbar_init(&peer_landed[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], 2 * kPairReaders);  // the epilogue warps of both CTAs
+        }
+        mbar_init(&done, 1);
+        abort_flag = g_int8_force_abort;
+        if (abort_flag) atomicCAS(&g_int8_error, 0, 2);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&tmem_base)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers exist before any remote arrival
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool alive = true;
+            for (int tile = blockIdx.x / 2; tile < tiles && alive; tile += pairs) {
+                const int n = (tile % ctiles) * 256 + static_cast<int>(rank) * 128;
+                const int m = (tile / ctiles) * 256 + static_cast<int>(rank) * 128;
+                for (int p = 0; p < 3 && alive; ++p) {
+                    const CUtensorMap* x = &maps.x[x_of(p)];
+                    const CUtensorMap* w = &maps.w[w_of(p)];
+                    for (int k = 0; k < kblocks; ++k, ++it) {
+                        const int s = it % kPairStages;
+                        if (*ab.flag || (it >= kPairStages &&
+                                         !mbar_wait(&empty[s], ((it / kPairStages) - 1) & 1, ab, 21))) {
+                            alive = false;
+                            break;
+                        }
+                        const uint32_t dst = smem_u32(smem + s * kPairStage);
+                        mbar_expect_tx(&landed[s], kPairStage);
+                        tma_load(dst, w, k * kBK, n, &landed[s]);
+                        tma_load(dst + 128 * kBK, x, k * kBK, m, &landed[s]);
+                    }
+                }
+            }
+            // copies still in flight (after an abort) land before the CTA may exit
+            for (int i = it > kPairStages ? it - kPairStages : 0; i < it; ++i)
+                if (!mbar_drain(&landed[i % kPairStages], (i / kPairStages) & 1))
+                    atomicCAS(&g_int8_error, 0, 23);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank != 0) {
+            // tells the leader which stages have landed here
+            const int my_tiles = (tiles - static_cast<int>(blockIdx.x / 2) + pairs - 1) / pairs;
+            const int iters = my_tiles * 3 * kblocks;
+            for (int it = 0; it < iters; ++it) {
+                const int s = it % kPairStages;
+                if (!mbar_wait(&landed[s], (it / kPairStages) & 1, ab, 22)) break;
+                arrive_cluster(map_to(smem_u32(&peer_landed[s]), 0));
+            }
+        } else if (lane == 0) {
+            int it = 0, unit = 0;
+            bool alive = true;
+            for (int tile = blockIdx.x / 2; tile < tiles && alive; tile += pairs) {
+                for (int p = 0; p < 3 && alive; ++p, ++unit) {
+                    const uint32_t idesc = instr_desc(p == 2, 256, 256);
+                    const int slot = unit & 1;
+                    if (unit >= 2 && !mbar_wait(&acc_empty[slot], ((unit / 2) - 1) & 1, ab, 24)) {
+                        alive = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d = tmem + slot * 256;
+                    for (int k = 0; k < kblocks; ++k, ++it) {
+                        const int s = it % kPairStages;
+                        const uint32_t par = (it / kPairStages) & 1;
+                        if (!mbar_wait(&landed[s], par, ab, 25) ||
+                            !mbar_wait(&peer_landed[s], par, ab, 26)) {
+                            alive = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t base = smem_u32(smem + s * kPairStage);
+                        const uint64_t a = tile_desc(base), b = tile_desc(base + 128 * kBK);
+#pragma unroll
+                        for (int j = 0; j < kBK / 32; ++j)
+                            mma_i8<true>(d, a + 2 * j, b + 2 * j, idesc, k == 0 && j == 0 ? 0u : 1u);
+                        mma_commit_pair(&empty[s]);
+                    }
+                    if (alive) mma_commit_pair(&acc_full[slot]);
+                }
+            }
+            mma_commit_pair(&done);
+        }
+    } else {
+        const int quarter = warp & 3, part = (warp - 2) >> 2;  // columns part * 64 .. + 63
+        const int t = threadIdx.x - 64;
+        const uint32_t lane0 = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t empty0 = map_to(smem_u32(&acc_empty[0]), 0);
+        // The scales and biases of a tile, copied while the tile before it is read.
+        auto fetch = [&](int tile, int buf) {
+            const int m0 = (tile / ctiles) * 256;
+            const int c0 = (tile % ctiles) * 256 + static_cast<int>(rank) * 128;
+            for (int i = t; i < 3 * 256; i += 32 * kPairReaders) {
+                const int m = m0 + (i & 255);
+                const bool read = tile < tiles && m < g.M;
+                copy4(&scale[buf][i >> 8][i & 255],
+                      read ? g.xs + static_cast<int64_t>(x_of(i >> 8)) * g.M + m : g.xs, read);
+            }
+            for (int i = t; i < 5 * 128; i += 32 * kPairReaders) {
+                const int q = i >> 7, c = c0 + (i & 127);
+                const float* src = q < 3 ? g.ws + static_cast<int64_t>(w_of(q)) * g.N
+                                         : (q == 3 ? g.Sb : g.mb);
+                const bool read = tile < tiles && c < g.N && src != nullptr;
+                copy4(&chan[buf][q][i & 127], read ? src + c : g.xs, read);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int unit = 0, buf = 0;
+        bool alive = true;
+        fetch(blockIdx.x / 2, 0);
+        for (int tile = blockIdx.x / 2; tile < tiles; tile += pairs, buf ^= 1) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            // every reader's copies are here, and all have left the other buffer
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kPairReaders) : "memory");
+            fetch(tile + pairs, buf ^ 1);
+            const int m0 = (tile / ctiles) * 256 + part * 64;
+            const int n = (tile % ctiles) * 256 + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+            const bool in = n < g.N;
+            const int lim = g.M - m0;  // columns that are tokens
+            const int ch = quarter * 32 + lane;
+            float first[64];
+#pragma unroll
+            for (int p = 0; p < 3; ++p, ++unit) {
+                const int slot = unit & 1;
+                if (alive)
+                    alive = __all_sync(0xffffffffu, mbar_wait(&acc_full[slot], (unit / 2) & 1, ab, 27));
+                if (!alive) break;
+                tc_fence_after();
+                const uint32_t t0 = tmem + lane0 + slot * 256 + part * 64;
+                const float4* sc = reinterpret_cast<const float4*>(&scale[buf][p][part * 64]);
+                const float b = chan[buf][p][ch], bias = chan[buf][p == 2 ? 4 : 3][ch];
+                const float b0 = chan[buf][0][ch];
+                float* out = (p == 2 ? g.mz : g.Sz) + static_cast<int64_t>(m0) * g.N + n;
+#pragma unroll
+                for (int c = 0; c < 64; c += 8) {  // 8 at a time: first[] leaves no room for more
+                    uint32_t r[8];
+                    tmem_ld8(t0 + c, r);
+                    const float4 s0 = sc[c / 4], s1 = sc[c / 4 + 1];
+                    const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+                    tmem_wait_ld();
+                    if (p == 0) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            first[c + e] = sv[e] * static_cast<float>(static_cast<int>(r[e]));
+                    } else {
+                        float z[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            z[e] = fmaf(sv[e] * static_cast<float>(static_cast<int>(r[e])), b,
+                                        p == 1 ? fmaf(first[c + e], b0, bias) : bias);
+                        if (in && c + 8 <= lim) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                *out = z[e];
+                                out += g.N;
+                            }
+                        } else if (in) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                if (c + e < lim) *out = z[e];
+                                out += g.N;
+                            }
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_cluster(empty0 + slot * 8);
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 1 && lane == 0 && !mbar_drain(&done, 0)) atomicCAS(&g_int8_error, 0, 28);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // no remote arrival or commit is still due
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ---- few tokens or few tiles: a tile's work shared out over a cluster ------------------
+constexpr int kSplitThreads = 192;
+
+template <int BN>
+struct Split {
+    static constexpr int STAGE = 128 * kBK + BN * kBK;
+    static constexpr int STAGES = 5;
+    static constexpr int COLS = 4 * BN;  // three accumulators; a power of 2
+    // the integer sums of the three products, for the exchange, use the stages' room
+    static_assert(3 * BN * 128 * 4 <= STAGES * STAGE, "the sums fit");
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+};
+
+// Work items of CTA `rank` of `ctas`: the list of (product, reduction block) cut evenly.
+__device__ __forceinline__ int share(int items, int rank, int ctas) {
+    return static_cast<int>(static_cast<int64_t>(items) * rank / ctas);
 }
 
 template <int BN>
-__global__ void __launch_bounds__(kThreads) int8_linear_kernel(const Int8Args g,
-                                                               const __grid_constant__ Maps maps) {
-    using P = Plan<BN>;
+__global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Args g,
+                                                                   const __grid_constant__ Maps maps) {
+    using P = Split<BN>;
     extern __shared__ char raw[];
     __shared__ __align__(8) uint64_t full[P::STAGES], empty[P::STAGES], done;
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag;
-    __shared__ float scale[2][BN];
+    __shared__ float scale[3][BN];
+    __shared__ int held[8];  // the products that CTA r has sums of, a bit each
     char* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * 128, m0 = blockIdx.y * BN;
-    const bool var = blockIdx.z == 0;
+    const int ctas = gridDim.z, rank = blockIdx.z;  // the cluster runs along z
     const int kblocks = (g.K + kBK - 1) / kBK;
-    const int iters = var ? 2 * kblocks : kblocks;
-    volatile int* ab = &abort_flag;
+    const int beg = share(3 * kblocks, rank, ctas), end = share(3 * kblocks, rank + 1, ctas);
+    const Abort ab{&abort_flag, 0};
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < P::STAGES; ++s) {
@@ -217,92 +534,145 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const Int8Args g,
 
     if (warp == 0) {
         if (lane == 0) {
-            int issued = 0;
-            for (int it = 0; it < iters; ++it) {
+            int it = 0;
+            for (int i = beg; i < end; ++i, ++it) {
                 const int s = it % P::STAGES;
-                if (*ab) break;
-                if (it >= P::STAGES && !mbar_wait(&empty[s], ((it / P::STAGES) - 1) & 1, ab, 11))
+                if (*ab.flag || (it >= P::STAGES &&
+                                 !mbar_wait(&empty[s], ((it / P::STAGES) - 1) & 1, ab, 11)))
                     break;
-                const bool second = it >= kblocks;
-                const int k = (second ? it - kblocks : it) * kBK;
-                // variance: x_2 with w_S, then x_S with w_2; mean: x_m with w_m
-                const CUtensorMap* x = &maps.x[var ? (second ? 2 : 1) : 0];
-                const CUtensorMap* w = &maps.w[var ? (second ? 1 : 2) : 0];
+                const int p = i / kblocks, k = (i - p * kblocks) * kBK;
                 const uint32_t dst = smem_u32(smem + s * P::STAGE);
                 mbar_expect_tx(&full[s], P::STAGE);
-                tma_load(dst, w, k, n0, &full[s]);
-                tma_load(dst + 128 * kBK, x, k, m0, &full[s]);
-                issued = it + 1;
+                tma_load(dst, &maps.w[w_of(p)], k, n0, &full[s]);
+                tma_load(dst + 128 * kBK, &maps.x[x_of(p)], k, m0, &full[s]);
             }
-            // copies still in flight (after an abort) land before the block may exit
-            for (int it = issued > P::STAGES ? issued - P::STAGES : 0; it < issued; ++it)
-                if (!mbar_drain(&full[it % P::STAGES], (it / P::STAGES) & 1))
+            // copies still in flight (after an abort) land before the CTA may exit
+            for (int i = it > P::STAGES ? it - P::STAGES : 0; i < it; ++i)
+                if (!mbar_drain(&full[i % P::STAGES], (i / P::STAGES) & 1))
                     atomicCAS(&g_int8_error, 0, 13);
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            const uint32_t idesc = instr_desc(!var, BN);
-            for (int it = 0; it < iters; ++it) {
+            for (int i = beg, it = 0; i < end; ++i, ++it) {
                 const int s = it % P::STAGES;
                 if (!mbar_wait(&full[s], (it / P::STAGES) & 1, ab, 12)) break;
                 tc_fence_after();
-                const bool second = it >= kblocks;
+                const int p = i / kblocks;
+                const uint32_t idesc = instr_desc(p == 2, 128, BN);
                 const uint32_t base = smem_u32(smem + s * P::STAGE);
                 const uint64_t a = tile_desc(base), b = tile_desc(base + 128 * kBK);
-                const uint32_t d = tmem + (second ? BN : 0);
-                const bool first = it == 0 || it == kblocks;
+                const bool first = i == beg || i == p * kblocks;
 #pragma unroll
-                for (int k = 0; k < kBK / 32; ++k)
-                    mma_i8(d, a + 2 * k, b + 2 * k, idesc, first && k == 0 ? 0u : 1u);
+                for (int j = 0; j < kBK / 32; ++j)
+                    mma_i8<false>(tmem + p * BN, a + 2 * j, b + 2 * j, idesc, first && j == 0 ? 0u : 1u);
                 mma_commit(&empty[s]);
             }
             mma_commit(&done);
         }
     } else {
         const int t = threadIdx.x - 64;
-        for (int i = t; i < 2 * BN; i += 128) {
-            const int c = i / BN, m = m0 + i % BN;
-            const int which = var ? (c == 0 ? 1 : 2) : 0;
-            scale[c][i % BN] = m < g.M ? g.xs[static_cast<int64_t>(which) * g.M + m] : 0.f;
+        if (t < ctas) {
+            const int lo = share(3 * kblocks, t, ctas), hi = share(3 * kblocks, t + 1, ctas);
+            int bits = 0;
+            for (int p = 0; p < 3; ++p)
+                if (lo < hi && hi > p * kblocks && lo < (p + 1) * kblocks) bits |= 1 << p;
+            held[t] = bits;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const int quarter = warp & 3;
-        const int n = n0 + quarter * 32 + lane;
-        float b0 = 0.f, b1 = 0.f, bias = 0.f;
+        for (int i = t; i < 3 * BN; i += 128) {
+            const int p = i / BN, m = m0 + i % BN;
+            scale[p][i % BN] = m < g.M ? g.xs[static_cast<int64_t>(x_of(p)) * g.M + m] : 0.f;
+        }
+    }
+    // accumulators: one thread per channel
+    const int quarter = warp & 3;
+    const int ch = quarter * 32 + lane, n = n0 + ch;
+    const bool reader = warp >= 2;
+    float b[3] = {0.f, 0.f, 0.f}, mb = 0.f, Sb = 0.f;
+    bool ok = false;
+    if (reader) {
         if (n < g.N) {
-            b0 = g.ws[(var ? 2 * static_cast<int64_t>(g.N) : 0) + n];
-            b1 = var ? g.ws[static_cast<int64_t>(g.N) + n] : 0.f;
-            const float* bp = var ? g.Sb : g.mb;
-            bias = bp ? bp[n] : 0.f;
-        }
-        float* out = var ? g.Sz : g.mz;
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, ab, 14) && !*ab);
-        if (ok) {
-            tc_fence_after();
-            const uint32_t t0 = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-#pragma unroll 1
-            for (int c = 0; c < BN; c += 16) {
-                if (m0 + c >= g.M) break;
-                uint32_t r0[16], r1[16];
-                tmem_ld16(t0 + c, r0);
-                if (var) tmem_ld16(t0 + BN + c, r1);
-                tmem_wait_ld();
-                if (n < g.N) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int m = m0 + c + e;
-                        if (m < g.M) {
-                            float z = scale[0][c + e] * b0 * static_cast<float>(static_cast<int>(r0[e]));
-                            if (var)
-                                z += scale[1][c + e] * b1 * static_cast<float>(static_cast<int>(r1[e]));
-                            out[static_cast<int64_t>(m) * g.N + n] = z + bias;
-                        }
-                    }
+            for (int p = 0; p < 3; ++p) b[p] = g.ws[static_cast<int64_t>(w_of(p)) * g.N + n];
+            mb = g.mb ? g.mb[n] : 0.f;
+            Sb = g.Sb ? g.Sb[n] : 0.f;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // scale[] and held[] are in place
+        ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, ab, 14) && !*ab.flag);
+        tc_fence_after();
+    }
+    const uint32_t t0 = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    auto put = [&](int c, int a0, int a1, int a2) {
+        const int m = m0 + c;
+        if (n >= g.N || m >= g.M) return;
+        const int64_t o = static_cast<int64_t>(m) * g.N + n;
+        g.Sz[o] = scale[0][c] * b[0] * static_cast<float>(a0) +
+                  scale[1][c] * b[1] * static_cast<float>(a1) + Sb;
+        g.mz[o] = scale[2][c] * b[2] * static_cast<float>(a2) + mb;
+    };
+    if (ctas == 1) {
+        if (ok) {
+#pragma unroll 1
+            for (int c = 0; c < BN && m0 + c < g.M; c += 16) {
+                uint32_t r0[16], r1[16], r2[16];
+                tmem_ld16(t0 + c, r0);
+                tmem_ld16(t0 + BN + c, r1);
+                tmem_ld16(t0 + 2 * BN + c, r2);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    put(c + e, static_cast<int>(r0[e]), static_cast<int>(r1[e]),
+                        static_cast<int>(r2[e]));
+            }
+        }
+    } else {
+        // every copy and MMA of this CTA is complete: its stages hold the sums now
+        int* sums = reinterpret_cast<int*>(smem);
+        if (reader && ok) {
+#pragma unroll 1
+            for (int p = 0; p < 3; ++p) {
+                if (!(held[rank] >> p & 1)) continue;
+#pragma unroll 1
+                for (int c = 0; c < BN; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(t0 + p * BN + c, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        sums[(p * BN + c + e) * 128 + ch] = static_cast<int>(r[e]);
                 }
             }
         }
-        tc_fence_before();
+        __syncwarp();
+        cluster_sync();
+        if (reader && ok) {
+            // this CTA adds the columns [c0, c1), kWide at a time: the remote loads of
+            // all CTAs that hold a product are in flight together
+            constexpr int kWide = BN >= 64 ? 4 : 2;
+            const int c0 = share(BN, rank, ctas), c1 = share(BN, rank + 1, ctas);
+            const uint32_t at0 = smem_u32(&sums[ch]);
+            for (int c = c0; c < c1; c += kWide) {
+                int a[3][kWide] = {};
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    if (r >= ctas) break;
+                    const uint32_t at = map_to(at0, r) + c * 512;
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        if (!(held[r] >> p & 1)) continue;
+#pragma unroll
+                        for (int i = 0; i < kWide; ++i)
+                            if (c + i < c1) a[p][i] += ld_cluster(at + (p * BN + i) * 512);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kWide; ++i)
+                    if (c + i < c1) put(c + i, a[0][i], a[1][i], a[2][i]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // the sums stay until every CTA has read them
     }
+    tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         if (lane == 0 && !mbar_drain(&done, 0)) atomicCAS(&g_int8_error, 0, 15);
@@ -346,22 +716,73 @@ bool encode(CUtensorMap* map, const void* p, int64_t rows, int64_t K, int64_t ld
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Which kernel, and how a tile of the split kernel is cut. Measured with cold inputs,
+// us with about 5 us of the measurement itself:
+//   pairs from 96 tiles of 128 x 128 on (32 pairs at work): 1024 x 2048 by K = 512 18
+//     against 26 split, 512 x 4096 by 1024 23 against 33; below, fewer pairs lose:
+//     2048 x 512 by 2048 32 against 29, 8192 x 128 by 512 20 against 17.
+//   BN: the narrowest tile that leaves at least three quarters of the SMs to the
+//     reduction's shares: 64 x 4096 by 4096 29 (64 columns, 4 shares) against 34 (16
+//     columns, 2 shares); 33 x 1000 by 1000 14 (16 columns, 4 shares) against 19 (64).
+//   shares: as many as the SMs hold, 4 blocks of the reduction each or more: 1 x 512
+//     by 2048 14 with 8, 25 with 1; 16 x 4096 by 4096 25 against 43. The exchange costs
+//     2 us (16 columns) to 4 us (64), so short reductions are not shared: 16 x 512 by
+//     512 13 whole, 14 in two; 256 x 1024 by 1024 20 whole, 21 in two or four.
+struct Route {
+    bool pair;
+    int bn, ctas;
+};
+Route route(int64_t M, int64_t N, int64_t K) {
+    const int64_t items = 3 * ((K + kBK - 1) / kBK), ntiles = (N + 127) / 128;
+    if (((M + 127) / 128) * ntiles >= 96) return {true, 256, 2};
+    Route r{false, 16, 1};
+    while (r.bn < 64 && ((M + r.bn - 1) / r.bn) * ntiles > kNumSMs / 4) r.bn *= 2;
+    const int64_t tiles = ((M + r.bn - 1) / r.bn) * ntiles;
+    if (items >= (r.bn == 64 ? 36 : 18))
+        while (r.ctas < 8 && tiles * r.ctas * 2 <= kNumSMs && items >= r.ctas * 8) r.ctas *= 2;
+    return r;
+}
+
+// The attribute belongs to the current device's copy of the kernel.
+template <typename K>
+int reserve_smem(K kernel, int bytes, const char* what) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) return TAGI_OK;
+    cudaGetLastError();
+    set_error("%s: cannot reserve %d bytes of shared memory (%s)", what, bytes,
+              cudaGetErrorString(e));
+    return TAGI_E_LAUNCH;
+}
+
+int launch_pair(const Int8Args& g, const Maps& maps, cudaStream_t st, const char* what) {
+    if (const int rc = reserve_smem(int8_pair_kernel, kPairSmem, what)) return rc;
+    const int64_t tiles = ((static_cast<int64_t>(g.M) + 255) / 256) * ((g.N + 255) / 256);
+    TAGI_REQUIRE(tiles <= INT32_MAX / 2, TAGI_E_UNSUPPORTED, "%s: too many tiles", what);
+    const int64_t pairs = tiles < kNumSMs / 2 ? tiles : kNumSMs / 2;
+    int8_pair_kernel<<<static_cast<unsigned>(2 * pairs), kPairThreads, kPairSmem, st>>>(g, maps);
+    count_tc_launch();
+    return check_launch(what);
+}
+
 template <int BN>
-int launch(const Int8Args& g, const Maps& maps, cudaStream_t st, const char* what) {
-    using P = Plan<BN>;
-    // the attribute belongs to the current device's copy of the kernel
-    const cudaError_t e = cudaFuncSetAttribute(
-        int8_linear_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::SMEM);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        set_error("%s: cannot reserve %d bytes of shared memory (%s)", what, P::SMEM,
-                  cudaGetErrorString(e));
-        return TAGI_E_LAUNCH;
-    }
+int launch_split(const Int8Args& g, const Maps& maps, int ctas, cudaStream_t st, const char* what) {
+    using P = Split<BN>;
+    if (const int rc = reserve_smem(int8_split_kernel<BN>, P::SMEM, what)) return rc;
     const int64_t my = (static_cast<int64_t>(g.M) + BN - 1) / BN;
     TAGI_REQUIRE(my <= 65535, TAGI_E_UNSUPPORTED, "%s: too many rows", what);
-    const dim3 grid((g.N + 127) / 128, static_cast<unsigned>(my), 2);
-    int8_linear_kernel<BN><<<grid, kThreads, P::SMEM, st>>>(g, maps);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((g.N + 127) / 128, static_cast<unsigned>(my), ctas);
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = P::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = cfg.gridDim.z;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, int8_split_kernel<BN>, g, maps);
     count_tc_launch();
     return check_launch(what);
 }
@@ -400,7 +821,7 @@ extern "C" int tagi_int8_moment_matmul(const int8_t* x_m, const uint8_t* x_2, co
                                        int64_t K, void* stream) {
     const char* what = "tagi_int8_moment_matmul";
     // 255 * 255 * K stays below 2^31
-    TAGI_REQUIRE(M >= 0 && N >= 0 && K >= 1 && M <= INT32_MAX && N <= INT32_MAX && K <= 33025,
+    TAGI_REQUIRE(M >= 0 && N >= 0 && K >= 1 && M <= (1 << 30) && N <= (1 << 30) && K <= 33025,
                  TAGI_E_BAD_ARG, "%s: bad sizes (the reduction may have 1 to 33025 terms)", what);
     if (M == 0 || N == 0) return TAGI_OK;
     TAGI_REQUIRE(x_m && x_2 && x_S && x_scales && w_m && w_2 && w_S && w_scales && mz && Sz,
@@ -414,17 +835,19 @@ extern "C" int tagi_int8_moment_matmul(const int8_t* x_m, const uint8_t* x_2, co
     TAGI_REQUIRE((bits & 15) == 0, TAGI_E_ALIGNMENT,
                  "%s: rows of codes must start on 16-byte boundaries", what);
     TAGI_REQUIRE(encode_tiled() != nullptr, TAGI_E_LAUNCH, "%s: no tensor-map encoder", what);
-    const int bn = M <= 16 ? 16 : (M <= 64 ? 64 : 128);
+    const Route r = route(M, N, K);
+    const int box = r.pair ? 128 : r.bn;
     Maps maps;
     const void* x[3] = {x_m, x_2, x_S};
     const void* w[3] = {w_m, w_2, w_S};
     for (int i = 0; i < 3; ++i)
-        TAGI_REQUIRE(encode(&maps.x[i], x[i], M, K, ldx, bn) && encode(&maps.w[i], w[i], N, K, ldw, 128),
+        TAGI_REQUIRE(encode(&maps.x[i], x[i], M, K, ldx, box) && encode(&maps.w[i], w[i], N, K, ldw, 128),
                      TAGI_E_LAUNCH, "%s: the tensor maps were refused", what);
     const Int8Args g{x_scales, w_scales, mb, Sb, mz, Sz, static_cast<int>(M), static_cast<int>(N),
                      static_cast<int>(K)};
     cudaStream_t st = as_stream(stream);
-    if (bn == 16) return launch<16>(g, maps, st, what);
-    if (bn == 64) return launch<64>(g, maps, st, what);
-    return launch<128>(g, maps, st, what);
+    if (r.pair) return launch_pair(g, maps, st, what);
+    if (r.bn == 16) return launch_split<16>(g, maps, r.ctas, st, what);
+    if (r.bn == 32) return launch_split<32>(g, maps, r.ctas, st, what);
+    return launch_split<64>(g, maps, r.ctas, st, what);
 }
