@@ -146,6 +146,31 @@ inline unsigned grid_1d(int64_t n, int threads, int64_t max_blocks = 148 * 16) {
     return static_cast<unsigned>(b);
 }
 
+// A kernel that continues the one before it in the stream: launched while that one
+// still runs (once all its blocks have called launch_dependents or ended), so that the
+// launch itself is hidden. It calls wait_for_primary() before it touches anything that
+// the one before it writes or reads; that returns when that kernel has ended and its
+// writes are visible.
+template <typename... P, typename... A>
+inline void launch_early(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+__device__ __forceinline__ void launch_dependents() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_primary() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 }  // namespace tagi
 
 #define TAGI_REQUIRE(cond, code, ...)  \

@@ -13,8 +13,9 @@
 //   reduce  1 launch.  Block (c, slice) walks the kChunk tokens of chunk c over
 //           its columns. A segment inside the chunk is finished at once; one that
 //           crosses a border leaves a partial sum (head: it began earlier; tail:
-//           it began here and goes on).
-//   join    1 launch.  The block of a chunk with a tail adds the heads that follow.
+//           it began here and goes on), and the chunk of a tail is put on a list.
+//           Further blocks zero the rows that no token names (sums, deltas).
+//   join    1 launch.  A block takes listed chunks and adds the heads that follow.
 //
 // Chunks are cut by position alone and partials are added in chunk order, so the
 // result does not depend on scheduling. A row's tokens are added in token order
@@ -104,32 +105,36 @@ __global__ void lookup_kernel(const void* ids, const float* mw, const float* Sw,
 }
 
 // ---- sort ---------------------------------------------------------------------
-constexpr int kSortThreads = 1024;
+constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kBins = 256;
-constexpr int kSortCluster = 8;  // the largest portable cluster
+constexpr int kSortCluster = 16;  // above the portable 8: scattered stores bind this kernel
+constexpr int kItems = 8;        // elements that a thread loads together
 
 struct SortArgs {
     const void* ids;
     int n, V, passes, bits;  // bits per pass
     int64_t pad;
-    int* key[2];
-    int* pos[2];
+    int2* list[2];  // (row, position)
+    int* listed;    // numbers of listed chunks, set to 0 here
 };
 
 // One cluster sorts (row, position) by row, stably: least significant digit first.
 // CTA r owns the r-th run of the list and each of its warps a run of that, so list
-// order is (CTA, warp, iteration, lane). Per pass: every warp counts its digits;
-// the counts become offsets (over warps inside the CTA, over CTAs through
-// distributed shared memory, over digits); every warp walks its run again and puts
-// each element at its digit's offset plus its rank among the equal digits of its
-// 32 lanes.
+// order is (CTA, warp, iteration, lane). Per pass: every warp counts its digits, and
+// an element's rank among the equal digits before it in the run falls out of the same
+// step (match over the 32 lanes plus the running count); the counts become offsets
+// (over warps inside the CTA, over CTAs through distributed shared memory, over
+// digits); every element goes to its digit's offset plus its rank. Runs of up to
+// 32 * kItems elements stay in registers between the two steps (65536 tokens in all);
+// longer ones are read and ranked again.
 template <int IDT>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a) {
     __shared__ int count[kSortWarps][kBins];
     __shared__ int total[kBins];   // this CTA's digit counts, read by the whole cluster
     __shared__ int start[kBins];
     __shared__ int warp_sum[kBins / 32];
+    launch_dependents();
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks());
     const int rank = static_cast<int>(cluster.block_rank());
@@ -140,30 +145,56 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
     const int lo = static_cast<int>(first < a.n ? first : a.n);
     const int hi = static_cast<int>(first + per < a.n ? first + per : a.n);
     const int mask = (1 << a.bits) - 1;
+    const bool single = per <= 32 * kItems;
+    if (rank == 0 && threadIdx.x < 2) a.listed[threadIdx.x] = 0;
 
     for (int pass = 0; pass < a.passes; ++pass) {
         const int shift = pass * a.bits;
-        const int* key = a.key[(pass + 1) & 1];
-        const int* pos = a.pos[(pass + 1) & 1];
-        int* key_out = a.key[pass & 1];
-        int* pos_out = a.pos[pass & 1];
-        auto key_at = [&](int i) {
-            if (pass > 0) return key[i];
-            const int v = row_of<IDT>(a.ids, i, a.V, a.pad);
-            return v < 0 ? a.V : v;
+        const int2* in_list = a.list[(pass + 1) & 1];
+        int2* out_list = a.list[pass & 1];
+        int k[kItems], p[kItems], off[kItems];
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int j = 0; j < kItems; ++j) {
+                const int i = i0 + 32 * j + lane;
+                if (i < hi) {
+                    if (pass > 0) {
+                        const int2 x = in_list[i];
+                        k[j] = x.x;
+                        p[j] = x.y;
+                    } else {
+                        const int v = row_of<IDT>(a.ids, i, a.V, a.pad);
+                        k[j] = v < 0 ? a.V : v;
+                        p[j] = i;
+                    }
+                }
+            }
+        };
+        // off = rank among the equal digits that the warp has counted so far
+        auto rank_items = [&](int i0) {
+#pragma unroll
+            for (int j = 0; j < kItems; ++j) {
+                if (i0 + 32 * j >= hi) break;
+                const bool in = i0 + 32 * j + lane < hi;
+                const int d = in ? (k[j] >> shift) & mask : kBins;
+                const unsigned same = __match_any_sync(0xffffffffu, d);
+                const int ahead = __popc(same & ((1u << lane) - 1u));
+                if (in) off[j] = count[warp][d] + ahead;
+                __syncwarp();
+                if (in && ahead == 0) count[warp][d] += __popc(same);
+                __syncwarp();
+            }
         };
         for (int b = lane; b < kBins; b += 32) count[warp][b] = 0;
         __syncwarp();
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            const int d = i < hi ? (key_at(i) >> shift) & mask : kBins;
-            const unsigned same = __match_any_sync(0xffffffffu, d);
-            if (d < kBins && (same & ((1u << lane) - 1u)) == 0) count[warp][d] += __popc(same);
-            __syncwarp();
+        for (int i0 = lo; i0 < hi; i0 += 32 * kItems) {
+            load(i0);
+            rank_items(i0);
         }
         __syncthreads();
         if (threadIdx.x < kBins) {
             int run = 0;
+#pragma unroll 8
             for (int w = 0; w < kSortWarps; ++w) {
                 const int c = count[w][threadIdx.x];
                 count[w][threadIdx.x] = run;
@@ -174,7 +205,9 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
         cluster.sync();
         if (threadIdx.x < kBins) {
             int before = 0, all = 0;
-            for (int r = 0; r < ctas; ++r) {
+#pragma unroll
+            for (int r = 0; r < kSortCluster; ++r) {
+                if (r >= ctas) break;
                 const int c = *cluster.map_shared_rank(&total[threadIdx.x], r);
                 if (r < rank) before += c;
                 all += c;
@@ -190,28 +223,25 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
         }
         __syncthreads();
         if (threadIdx.x < kBins) {
-            int add = start[threadIdx.x];
+            int add = 0;
             for (int w = 0; w < warp; ++w) add += warp_sum[w];
-            for (int w = 0; w < kSortWarps; ++w) count[w][threadIdx.x] += add;
+            start[threadIdx.x] += add;
         }
         __syncthreads();
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            int k = 0, d = kBins;
-            if (i < hi) {
-                k = key_at(i);
-                d = (k >> shift) & mask;
+        for (int i0 = lo; i0 < hi; i0 += 32 * kItems) {
+            if (!single) {
+                load(i0);
+                rank_items(i0);
             }
-            const unsigned same = __match_any_sync(0xffffffffu, d);
-            const int ahead = __popc(same & ((1u << lane) - 1u));
-            if (i < hi) {
-                const int at = count[warp][d] + ahead;
-                key_out[at] = k;
-                pos_out[at] = pass > 0 ? pos[i] : i;
+#pragma unroll
+            for (int j = 0; j < kItems; ++j) {
+                const int i = i0 + 32 * j + lane;
+                if (i < hi) {
+                    const int d = (k[j] >> shift) & mask;
+                    const int at = start[d] + off[j] + (single ? count[warp][d] : 0);
+                    out_list[at] = make_int2(k[j], p[j]);
+                }
             }
-            __syncwarp();
-            if (i < hi && ahead == 0) count[warp][d] += __popc(same);
-            __syncwarp();
         }
         // the list of this pass is complete and every CTA has read the others'
         // totals before either is touched again
@@ -221,46 +251,65 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
 
 // ---- sums over the segments ------------------------------------------------------
 constexpr int kChunk = 32;    // sorted tokens per block
-constexpr int kAhead = 8;     // delta rows loaded ahead of the adds
-constexpr int kThreads = 128;
+constexpr int kThreads = 256; // columns' threads per block, at most
+constexpr int kGroups = 8;    // warps that share a long segment
+constexpr int kLong = 16;     // a segment is long when it goes on over so many chunks
 
 struct GradArgs {
-    const int* key;
-    const int* pos;
+    const int2* tok;  // sorted (row, position)
     const float* dm;
     const float* dS;
-    int n, V, D, mode;
-    float s, s2, cap;
+    int n, V, D;
+    float s, s2, inv_cap;
     float* mw;        // update: the table; deltas: Sw only
     float* Sw;
     float* out_m;     // sums and deltas
     float* out_S;
     float* part;      // [chunk][head m, head S, tail m, tail S][D]
+    int* listed;      // numbers of short and of long entries
+    int4* list;       // (first chunk, last chunk, row) of the segments that cross a border:
+                      // short ones from the front, long ones from the back
+    int chunks;
 };
 
-// The sums of one row's columns j..j+VEC-1 in their final form.
-template <int VEC, typename T>
-__device__ __forceinline__ void finish(const GradArgs& a, int v, int j, const T (&m)[VEC],
-                                       const T (&S)[VEC]) {
-    const int64_t o = static_cast<int64_t>(v) * a.D + j;
+// The capped update of capped_pair (common.cuh) with the division by the cap as a
+// product; a delta that is not a number leaves its parameter as it is, as there.
+__device__ __forceinline__ void capped_step(float& m, float& S, float dm, float dS, float inv_cap) {
+    const float bound = sqrtf(fmaxf(S, 1e-10f)) * inv_cap;
+    m += dm == dm ? fminf(fmaxf(dm, -bound), bound) : 0.f;
+    const float raw = S + (dS == dS ? fminf(fmaxf(dS, -bound), bound) : 0.f);
+    S = raw <= 0.f ? 1e-5f : raw;
+}
+
+// The row's parameters that the final form needs.
+template <int VEC, int MODE>
+__device__ __forceinline__ void params(const GradArgs& a, int64_t o, float (&mean)[VEC],
+                                       float (&w)[VEC]) {
+    using T = typename Vec<VEC>::type;
+    if (MODE != TAGI_WGRAD_SUMS) *reinterpret_cast<T*>(w) = *reinterpret_cast<const T*>(a.Sw + o);
+    if (MODE == TAGI_WGRAD_UPDATE)
+        *reinterpret_cast<T*>(mean) = *reinterpret_cast<const T*>(a.mw + o);
+}
+
+// The sums of one row at offset o in their final form.
+template <int VEC, int MODE, typename T>
+__device__ __forceinline__ void finish(const GradArgs& a, int64_t o, const T (&m)[VEC],
+                                       const T (&S)[VEC], float (&mean)[VEC], float (&w)[VEC]) {
     float gm[VEC], gS[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         gm[e] = static_cast<float>(m[e] * a.s);
         gS[e] = static_cast<float>(S[e] * a.s2);
     }
-    if (a.mode != TAGI_WGRAD_SUMS) {
-        float w[VEC];
-        ldv<VEC>(a.Sw + o, w);
-        if (a.mode == TAGI_WGRAD_UPDATE) {
-            float mean[VEC];
-            ldv<VEC>(a.mw + o, mean);
+    if (MODE == TAGI_WGRAD_UPDATE) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) capped_pair(mean[e], w[e], w[e] * gm[e], w[e] * w[e] * gS[e], a.cap);
-            stv<VEC>(a.mw + o, mean);
-            stv<VEC>(a.Sw + o, w);
-            return;
-        }
+        for (int e = 0; e < VEC; ++e)
+            capped_step(mean[e], w[e], w[e] * gm[e], w[e] * w[e] * gS[e], a.inv_cap);
+        stv<VEC>(a.mw + o, mean);
+        stv<VEC>(a.Sw + o, w);
+        return;
+    }
+    if (MODE == TAGI_WGRAD_DELTAS) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             gm[e] *= w[e];
@@ -271,154 +320,208 @@ __device__ __forceinline__ void finish(const GradArgs& a, int v, int j, const T 
     stv<VEC>(a.out_S + o, gS);
 }
 
+// Rows [32 * block * warps, ...) that no token names get zero sums: every lane looks
+// its row up in the sorted list, then the warp writes the absent ones.
 template <int VEC>
+__device__ __forceinline__ void zero_rows(const GradArgs& a, int block) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int64_t v0 = (static_cast<int64_t>(block) * warps + (threadIdx.x >> 5)) * 32;
+    const int64_t v = v0 + lane;
+    bool absent = false;
+    if (v < a.V) {
+        int lo = 0, hi = a.n;  // first token whose row is >= v
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (a.tok[mid].x < v) lo = mid + 1;
+            else hi = mid;
+        }
+        absent = lo == a.n || a.tok[lo].x != v;
+    }
+    float zero[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
+    for (unsigned rows = __ballot_sync(0xffffffffu, absent); rows != 0; rows &= rows - 1) {
+        const int64_t o = (v0 + __ffs(rows) - 1) * a.D;
+        for (int j = lane * VEC; j < a.D; j += 32 * VEC) {
+            stv<VEC>(a.out_m + o + j, zero);
+            stv<VEC>(a.out_S + o + j, zero);
+        }
+    }
+}
+
+// What happens to the running sum behind a token.
+enum { GOES_ON = 0, FINAL = 1, HEAD = 2, TAIL = 3 };
+
+// AHEAD tokens' delta rows, and the parameters of the rows that end among them, are
+// loaded before any of them is added: a row of one token (most rows of a text batch)
+// would otherwise wait for its parameters alone.
+template <int VEC, int MODE>
 __global__ void __launch_bounds__(kThreads) reduce_kernel(const GradArgs a) {
-    __shared__ int key[kChunk + 2];  // with the neighbours on both sides (-1: none)
-    __shared__ int pos[kChunk];
+    constexpr int AHEAD = 4;  // 8 cost occupancy: 19.2 us instead of 16.0 for 16384 x 512
+    __shared__ int4 tok[kChunk];  // row, position, what happens behind it
+    launch_dependents();
+    wait_for_primary();  // the sorted list
+    if (static_cast<int>(blockIdx.x) >= a.chunks) {
+        if (blockIdx.y == 0) zero_rows<VEC>(a, blockIdx.x - a.chunks);
+        return;
+    }
     const int c0 = blockIdx.x * kChunk;
-    const int cnt = min(kChunk, a.n - c0);
-    for (int i = threadIdx.x; i < cnt + 2; i += kThreads) {
-        const int t = c0 + i - 1;
-        key[i] = t >= 0 && t < a.n ? a.key[t] : -1;
-        if (i >= 1 && i <= cnt) pos[i - 1] = a.pos[t];
+    int cnt = min(kChunk, a.n - c0);
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        static_assert(kChunk == 32, "a lane per token");
+        const int t = c0 + lane;
+        const int2 x = t < a.n ? a.tok[t] : make_int2(a.V, 0);
+        const int prev = c0 > 0 ? a.tok[c0 - 1].x : -1;
+        int next = __shfl_down_sync(0xffffffffu, x.x, 1);
+        if (lane == 31) next = t + 1 < a.n ? a.tok[t + 1].x : -1;
+        const bool ends = next != x.x || lane == 31;
+        const bool after = lane == 31 && next == x.x, before = x.x == prev;
+        tok[lane] = make_int4(x.x, x.y, !ends ? GOES_ON : (before ? HEAD : (after ? TAIL : FINAL)), 0);
+        if (after && !before && x.x < a.V && blockIdx.y == 0) {
+            // a segment begins here and goes on: look for its last chunk
+            int last = blockIdx.x + 1, hi = a.chunks - 1;
+            for (int step = 1; last < hi;) {  // chunk k begins with this row: true up to the last
+                const int k = min(last + step, hi);
+                if (a.tok[static_cast<int64_t>(k) * kChunk].x == x.x) {
+                    last = k;
+                    step *= 2;
+                } else {
+                    hi = k - 1;
+                    step = max(1, (hi - last + 1) / 2);
+                }
+            }
+            const bool longer = last - static_cast<int>(blockIdx.x) >= kLong;
+            const int at = atomicAdd(&a.listed[longer], 1);
+            a.list[longer ? a.chunks - 1 - at : at] = make_int4(blockIdx.x, last, x.x, 0);
+        }
     }
     __syncthreads();
-    const int j = (blockIdx.y * kThreads + threadIdx.x) * VEC;
-    if (j >= a.D || key[1] == a.V) return;  // dropped tokens sort last
+    const int j = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    if (j >= a.D) return;
     float m[VEC], S[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) m[e] = S[e] = 0.f;
-    int seg = 0;  // first token of the running segment
-    for (int i0 = 0; i0 < cnt; i0 += kAhead) {
-        float xm[kAhead][VEC], xS[kAhead][VEC];
+    for (int i0 = 0; i0 < cnt; i0 += AHEAD) {
+        if (tok[i0].x >= a.V) break;  // dropped tokens sort last
+        float xm[AHEAD][VEC], xS[AHEAD][VEC], mean[AHEAD][VEC], w[AHEAD][VEC];
+        int row[AHEAD], kind[AHEAD];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (i0 + u < cnt && key[i0 + u + 1] < a.V) {
-                const int64_t o = static_cast<int64_t>(pos[i0 + u]) * a.D + j;
+        for (int u = 0; u < AHEAD; ++u) {
+            const int4 t = tok[i0 + u];
+            row[u] = t.x;
+            kind[u] = i0 + u < cnt && t.x < a.V ? t.z : -1;
+            if (kind[u] >= 0) {
+                const int64_t o = static_cast<int64_t>(t.y) * a.D + j;
                 ldv<VEC>(a.dm + o, xm[u]);
                 ldv<VEC>(a.dS + o, xS[u]);
             }
+            if (kind[u] == FINAL)
+                params<VEC, MODE>(a, static_cast<int64_t>(t.x) * a.D + j, mean[u], w[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int i = i0 + u;
-            if (i >= cnt || key[i + 1] >= a.V) break;
+        for (int u = 0; u < AHEAD; ++u) {
+            if (kind[u] < 0) break;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 m[e] += xm[u][e];
                 S[e] += xS[u][e];
             }
-            const int v = key[i + 1];
-            const bool last = i == cnt - 1;
-            if (!last && key[i + 2] == v) continue;
-            const bool before = seg == 0 && key[0] == v, after = last && key[i + 2] == v;
-            if (!before && !after) {
-                finish<VEC>(a, v, j, m, S);
+            if (kind[u] == GOES_ON) continue;
+            if (kind[u] == FINAL) {
+                finish<VEC, MODE>(a, static_cast<int64_t>(row[u]) * a.D + j, m, S, mean[u], w[u]);
             } else {
-                float* p = a.part + (static_cast<int64_t>(blockIdx.x) * 4 + (before ? 0 : 2)) * a.D;
+                float* p = a.part +
+                           (static_cast<int64_t>(blockIdx.x) * 4 + (kind[u] == HEAD ? 0 : 2)) * a.D;
                 stv<VEC>(p + j, m);
                 stv<VEC>(p + a.D + j, S);
             }
-            seg = i + 1;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) m[e] = S[e] = 0.f;
         }
     }
 }
 
-// Block (c, slice): if a segment begins in chunk c and goes on behind it, the sum
-// of its tail and of the heads of the chunks that it reaches. kGroups threads share
-// a column, each takes every kGroups-th chunk, and their sums are added in order.
-constexpr int kGroups = 8;
+// Adds the partials of chunks c, c + step, ... <= last of the segment that begins in
+// chunk `begin`, columns j..
 template <int VEC>
-__global__ void __launch_bounds__(32 * kGroups) join_kernel(const GradArgs a) {
-    __shared__ double sum[2][kGroups][32 * VEC];
-    const int c = blockIdx.x;
-    const int end = (c + 1) * kChunk;
-    if (end >= a.n) return;
-    const int v = a.key[end - 1];
-    if (v == a.V || a.key[end] != v) return;
-    const int c0 = c * kChunk;
-    if (c0 > 0 && a.key[c0] == v && a.key[c0 - 1] == v) return;  // began in an earlier chunk
-    int last = c + 1;  // the last chunk that the segment reaches
-    {
-        int lo = c + 1, hi = (a.n - 1) / kChunk;
-        while (lo < hi) {  // chunk k begins with v: true up to the last
-            const int mid = (lo + hi + 1) / 2;
-            if (a.key[mid * kChunk] == v) lo = mid;
-            else hi = mid - 1;
-        }
-        last = lo;
-    }
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int j = (blockIdx.y * 32 + lane) * VEC;
-    double m[VEC], S[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) m[e] = S[e] = 0.0;
-    if (j < a.D) {
+__device__ __forceinline__ void add_partials(const GradArgs& a, int begin, int c, int step, int last,
+                                             int j, double (&m)[VEC], double (&S)[VEC]) {
 #pragma unroll 4
-        for (int k = c + g; k <= last; k += kGroups) {
-            const float* p = a.part + (static_cast<int64_t>(k) * 4 + (k == c ? 2 : 0)) * a.D;
-            float x[VEC], y[VEC];
-            ldv<VEC>(p + j, x);
-            ldv<VEC>(p + a.D + j, y);
+    for (int k = c; k <= last; k += step) {
+        const float* p = a.part + (static_cast<int64_t>(k) * 4 + (k == begin ? 2 : 0)) * a.D;
+        float x[VEC], y[VEC];
+        ldv<VEC>(p + j, x);
+        ldv<VEC>(p + a.D + j, y);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                m[e] += x[e];
-                S[e] += y[e];
-            }
+        for (int e = 0; e < VEC; ++e) {
+            m[e] += x[e];
+            S[e] += y[e];
         }
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        sum[0][g][lane * VEC + e] = m[e];
-        sum[1][g][lane * VEC + e] = S[e];
-    }
-    __syncthreads();
-    if (g != 0 || j >= a.D) return;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        for (int k = 1; k < kGroups; ++k) {
-            m[e] += sum[0][k][lane * VEC + e];
-            S[e] += sum[1][k][lane * VEC + e];
-        }
-    }
-    finish<VEC>(a, v, j, m, S);
 }
 
-// Rows that no token names get zero sums: one warp per row looks it up in the
-// sorted list.
-template <int VEC>
-__global__ void absent_rows_kernel(const GradArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-    float zero[VEC];
+// Segments that cross a border: the tail of the chunk in which one begins and the heads
+// of those that it reaches. A warp takes the columns of a short one; for a long one
+// kGroups warps share them, each takes every kGroups-th chunk, and their sums are added
+// in order.
+template <int VEC, int MODE>
+__global__ void __launch_bounds__(32 * kGroups) join_kernel(const GradArgs a) {
+    __shared__ double sum[2][kGroups][32 * VEC];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int cols = (a.D + 32 * VEC - 1) / (32 * VEC);
+    wait_for_primary();  // the partials and the list of segments
+    const int shorts = a.listed[0], longs = a.listed[1];
+    for (int64_t it = static_cast<int64_t>(blockIdx.x) * kGroups + g;
+         it < static_cast<int64_t>(shorts) * cols; it += static_cast<int64_t>(gridDim.x) * kGroups) {
+        const int j = (static_cast<int>(it % cols) * 32 + lane) * VEC;
+        if (j >= a.D) continue;
+        const int4 c = a.list[it / cols];
+        const int64_t o = static_cast<int64_t>(c.z) * a.D + j;
+        double m[VEC] = {}, S[VEC] = {};
+        float mean[VEC], w[VEC];
+        add_partials<VEC>(a, c.x, c.x, 1, c.y, j, m, S);
+        params<VEC, MODE>(a, o, mean, w);
+        finish<VEC, MODE>(a, o, m, S, mean, w);
+    }
+    for (int64_t it = blockIdx.x; it < static_cast<int64_t>(longs) * cols; it += gridDim.x) {
+        const int4 c = a.list[a.chunks - 1 - it / cols];
+        const int j = (static_cast<int>(it % cols) * 32 + lane) * VEC;
+        const int64_t o = static_cast<int64_t>(c.z) * a.D + j;
+        double m[VEC] = {}, S[VEC] = {};
+        if (j < a.D) add_partials<VEC>(a, c.x, c.x + g, kGroups, c.y, j, m, S);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
-    for (int64_t v = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5; v < a.V;
-         v += warps) {
-        int lo = 0, hi = a.n;  // first token whose row is >= v
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (a.key[mid] < v) lo = mid + 1;
-            else hi = mid;
+        for (int e = 0; e < VEC; ++e) {
+            sum[0][g][lane * VEC + e] = m[e];
+            sum[1][g][lane * VEC + e] = S[e];
         }
-        if (lo < a.n && a.key[lo] == v) continue;
-        for (int j = lane * VEC; j < a.D; j += 32 * VEC) {
-            stv<VEC>(a.out_m + v * a.D + j, zero);
-            stv<VEC>(a.out_S + v * a.D + j, zero);
+        __syncthreads();
+        if (g == 0 && j < a.D) {
+            float mean[VEC], w[VEC];
+            params<VEC, MODE>(a, o, mean, w);
+            for (int k = 1; k < kGroups; ++k) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    m[e] += sum[0][k][lane * VEC + e];
+                    S[e] += sum[1][k][lane * VEC + e];
+                }
+            }
+            finish<VEC, MODE>(a, o, m, S, mean, w);
         }
+        __syncthreads();  // the sums are rewritten for the next segment
     }
 }
 
 size_t align_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-size_t list_bytes(int64_t n) { return align_up(static_cast<size_t>(n) * 4); }
+size_t list_bytes(int64_t n) { return align_up(static_cast<size_t>(n) * sizeof(int2)); }
 
 size_t grad_ws(int64_t n, int64_t D) {
     if (n <= 0) return 0;
     const size_t chunks = static_cast<size_t>((n + kChunk - 1) / kChunk);
-    return 4 * list_bytes(n) + align_up(chunks * 4 * static_cast<size_t>(D) * sizeof(float));
+    // the sorted list twice, the list of segments and its lengths, the partial sums
+    return 2 * list_bytes(n) + align_up((chunks + 1) * sizeof(int4)) +
+           align_up(chunks * 4 * static_cast<size_t>(D) * sizeof(float));
 }
 
 // The widest vectors that every row of every operand allows.
@@ -431,9 +534,17 @@ uintptr_t bits_of(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 template <int IDT>
 int launch_sort(const SortArgs& a, cudaStream_t st, const char* what) {
-    // a CTA takes 2048 tokens or more, so that small batches skip the cluster barriers
+    // a CTA takes 1024 tokens or more, so that small batches skip the cluster barriers
     int ctas = 1;
-    while (ctas < kSortCluster && a.n > ctas * 2048) ctas *= 2;
+    while (ctas < kSortCluster && a.n > ctas * 1024) ctas *= 2;
+    // the attribute belongs to the current device's copy of the kernel
+    const cudaError_t e =
+        cudaFuncSetAttribute(sort_kernel<IDT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        set_error("%s: clusters of %d refused (%s)", what, kSortCluster, cudaGetErrorString(e));
+        return TAGI_E_LAUNCH;
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kSortThreads);
@@ -448,22 +559,32 @@ int launch_sort(const SortArgs& a, cudaStream_t st, const char* what) {
     return check_launch(what);
 }
 
-template <int VEC>
-int launch_grad(const GradArgs& a, cudaStream_t st, const char* what) {
-    int rc;
-    if (a.mode != TAGI_WGRAD_UPDATE) {
-        absent_rows_kernel<VEC><<<grid_1d(static_cast<int64_t>(a.V) * 32, 256), 256, 0, st>>>(a);
-        if ((rc = check_launch(what))) return rc;
-    }
-    if (a.n == 0) return TAGI_OK;
-    const unsigned chunks = static_cast<unsigned>((a.n + kChunk - 1) / kChunk);
-    const int per = kThreads * VEC;
-    reduce_kernel<VEC><<<dim3(chunks, (a.D + per - 1) / per), kThreads, 0, st>>>(a);
-    if ((rc = check_launch(what))) return rc;
-    if (chunks == 1) return TAGI_OK;
-    const int jper = 32 * VEC;
-    join_kernel<VEC><<<dim3(chunks - 1, (a.D + jper - 1) / jper), 32 * kGroups, 0, st>>>(a);
+template <int VEC, int MODE>
+int launch_grad(GradArgs a, cudaStream_t st, const char* what) {
+    // the columns in even slices of whole warps
+    const int vecs = (a.D + VEC - 1) / VEC;
+    const int slices = (vecs + kThreads - 1) / kThreads;
+    const int threads = ((vecs + slices - 1) / slices + 31) / 32 * 32;
+    a.chunks = (a.n + kChunk - 1) / kChunk;
+    int64_t zero = 0;
+    if (MODE != TAGI_WGRAD_UPDATE) zero = (static_cast<int64_t>(a.V) + threads - 1) / threads;
+    if (a.chunks + zero == 0) return TAGI_OK;
+    TAGI_REQUIRE(a.chunks + zero <= INT32_MAX, TAGI_E_UNSUPPORTED, "%s: sizes beyond the grid", what);
+    const dim3 grid(static_cast<unsigned>(a.chunks + zero), slices);
+    launch_early(reduce_kernel<VEC, MODE>, grid, dim3(threads), st, a);
+    const int rc = check_launch(what);
+    if (rc || a.chunks <= 1) return rc;
+    const int64_t items = (static_cast<int64_t>(a.chunks - 1) * ((vecs + 31) / 32) + kGroups - 1) / kGroups;
+    launch_early(join_kernel<VEC, MODE>, dim3(grid_1d(items, 1, kNumSMs * 8)), dim3(32 * kGroups), st,
+                 a);
     return check_launch(what);
+}
+
+template <int VEC>
+int launch_mode(const GradArgs& a, int mode, cudaStream_t st, const char* what) {
+    if (mode == TAGI_WGRAD_SUMS) return launch_grad<VEC, TAGI_WGRAD_SUMS>(a, st, what);
+    if (mode == TAGI_WGRAD_DELTAS) return launch_grad<VEC, TAGI_WGRAD_DELTAS>(a, st, what);
+    return launch_grad<VEC, TAGI_WGRAD_UPDATE>(a, st, what);
 }
 
 }  // namespace
@@ -531,10 +652,12 @@ extern "C" int tagi_embedding_grad(const void* ids, int id_type, const float* dm
     if (n > 0) {
         SortArgs a{};
         char* w = static_cast<char*>(workspace);
-        for (int i = 0; i < 2; ++i) {
-            a.key[i] = reinterpret_cast<int*>(w + (2 * i) * list_bytes(n));
-            a.pos[i] = reinterpret_cast<int*>(w + (2 * i + 1) * list_bytes(n));
-        }
+        for (int i = 0; i < 2; ++i) a.list[i] = reinterpret_cast<int2*>(w + i * list_bytes(n));
+        const size_t chunks = static_cast<size_t>((n + kChunk - 1) / kChunk);
+        g.listed = a.listed = reinterpret_cast<int*>(w + 2 * list_bytes(n));
+        g.list = reinterpret_cast<int4*>(a.listed) + 1;
+        g.part = reinterpret_cast<float*>(w + 2 * list_bytes(n) +
+                                          align_up((chunks + 1) * sizeof(int4)));
         a.ids = ids;
         a.n = static_cast<int>(n);
         a.V = static_cast<int>(V);
@@ -547,26 +670,23 @@ extern "C" int tagi_embedding_grad(const void* ids, int id_type, const float* dm
                        : id_type == ID_I32 ? launch_sort<ID_I32>(a, st, what)
                                            : launch_sort<ID_I64>(a, st, what);
         if (rc) return rc;
-        g.key = a.key[(a.passes - 1) & 1];
-        g.pos = a.pos[(a.passes - 1) & 1];
-        g.part = reinterpret_cast<float*>(w + 4 * list_bytes(n));
+        g.tok = a.list[(a.passes - 1) & 1];
     }
     g.dm = dmz;
     g.dS = dSz;
     g.n = static_cast<int>(n);
     g.V = static_cast<int>(V);
     g.D = static_cast<int>(D);
-    g.mode = mode;
     g.s = scale;
     g.s2 = scale * scale;
-    g.cap = cap_factor;
+    g.inv_cap = 1.0f / cap_factor;
     g.mw = mw;
     g.Sw = Sw;
     g.out_m = out_m;
     g.out_S = out_S;
     const int vec = vec_of(D, bits_of(dmz) | bits_of(dSz) | bits_of(mw) | bits_of(Sw) |
                                   bits_of(out_m) | bits_of(out_S));
-    if (vec == 4) return launch_grad<4>(g, st, what);
-    if (vec == 2) return launch_grad<2>(g, st, what);
-    return launch_grad<1>(g, st, what);
+    if (vec == 4) return launch_mode<4>(g, mode, st, what);
+    if (vec == 2) return launch_mode<2>(g, mode, st, what);
+    return launch_mode<1>(g, mode, st, what);
 }

@@ -472,6 +472,7 @@ struct BackArgs {
 
 template <int VEC>
 __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackArgs g) {
+    launch_dependents();
     const int j = (blockIdx.y * kBackThreads + threadIdx.x) * VEC;
     if (j >= g.ni) return;
     const int64_t r0 = static_cast<int64_t>(blockIdx.x) * g.slice_rows;
@@ -525,6 +526,7 @@ __global__ void __launch_bounds__(256) back_finish_kernel(const double* part, in
     const int c = threadIdx.x & 7, g = threadIdx.x >> 3;
     const int col = blockIdx.x * 8 + c;
     double a = 0.0, b = 0.0;
+    wait_for_primary();  // the slices' sums
     if (col < ni) {
 #pragma unroll 8
         for (int s = g; s < slices; s += 32) {
@@ -717,7 +719,8 @@ extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, con
         back_kernel<1><<<grid, kBackThreads, 0, st>>>(g);
     const int rc = check_launch(what);
     if (rc) return rc;
-    back_finish_kernel<<<static_cast<unsigned>((ni + 7) / 8), 256, 0, st>>>(
-        g.part, slices, g.ni, mode, sums, mw, Sw, d_mw, d_Sw, cap_factor);
+    launch_early(back_finish_kernel, dim3(static_cast<unsigned>((ni + 7) / 8)), dim3(256), st,
+                 static_cast<const double*>(g.part), slices, g.ni, mode, sums, mw, Sw, d_mw, d_Sw,
+                 cap_factor);
     return check_launch(what);
 }
