@@ -85,30 +85,36 @@ __device__ __forceinline__ unsigned mag(float x) { return __float_as_uint(x) & 0
 __device__ __forceinline__ unsigned mag_pos(float x) { return x < 0.f ? 0u : mag(x); }
 constexpr unsigned kInfBits = 0x7f800000u;
 
-template <int WARPS>
-__device__ __forceinline__ float block_sum(float x, float* red) {
+// What a row is reduced to: sum of m^2 + S, largest |p|, t and (weights) u as keys. One
+// barrier for all of them, and sums in a fixed order.
+struct RowStats {
+    float sum;
+    unsigned P, T, U;
+};
+template <int OUT, int WARPS>
+__device__ __forceinline__ void reduce_row(RowStats& r, RowStats* red) {
+    constexpr bool NORM = OUT == OUT_F32 || OUT == OUT_INT8, CODES = OUT != OUT_F32;
+    if (NORM) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if (WARPS == 1) return x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (lane == 0) red[warp] = x;
+        for (int o = 16; o > 0; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
+    }
+    if (CODES) {
+        r.P = __reduce_max_sync(0xffffffffu, r.P);
+        r.T = __reduce_max_sync(0xffffffffu, r.T);
+        if (OUT == OUT_QUANT_W) r.U = __reduce_max_sync(0xffffffffu, r.U);
+    }
+    if (WARPS == 1) return;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = r;
     __syncthreads();
-    float s = 0.f;
+    r = red[0];
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) s += red[i];
-    return s;
-}
-template <int WARPS>
-__device__ __forceinline__ unsigned block_max(unsigned x, unsigned* red) {
-    x = __reduce_max_sync(0xffffffffu, x);
-    if (WARPS == 1) return x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (lane == 0) red[warp] = x;
-    __syncthreads();
-    unsigned s = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) s = max(s, red[i]);
-    return s;
+    for (int i = 1; i < WARPS; ++i) {
+        const RowStats o = red[i];
+        r.sum += o.sum;
+        r.P = max(r.P, o.P);
+        r.T = max(r.T, o.T);
+        r.U = max(r.U, o.U);
+    }
 }
 
 // p, t and (weights) u = m^2 + S of one element, in double: products of two fp32
@@ -187,8 +193,7 @@ __device__ __forceinline__ void codes(const Elem<OUT>& e, const RowScales& r, in
 // group has vectors i, i + 32 WARPS, ... (NV at most).
 template <int OUT, int VEC, int WARPS, int NV>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) row_kernel(const NormArgs g) {
-    __shared__ float red_f[WARPS];
-    __shared__ unsigned red_u[3][WARPS];
+    __shared__ RowStats red[WARPS];
     constexpr int T = 32 * WARPS;
     const int64_t row = WARPS == 1
                             ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5)
@@ -224,16 +229,32 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) row_kernel(cons
             }
         }
     }
+    RowStats rs{0.f, 0u, 0u, 0u};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int j = i0 + k * T * VEC;
+        if (j < g.ni) {
+            float w[VEC] = {}, sw[VEC] = {};
+            if (OUT == OUT_INT8) {
+                ld<VEC>(g.w + j, w);
+                ld<VEC>(g.Sw + j, sw);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (NORM) rs.sum += fmaf(m[k][e], m[k][e], S[k][e]);
+                if (OUT != OUT_F32) {
+                    const Elem<OUT> el(m[k][e], S[k][e], w[e], sw[e]);
+                    rs.P = max(rs.P, mag(static_cast<float>(el.p)));
+                    rs.T = max(rs.T, mag_pos(static_cast<float>(el.t)));
+                    if (OUT == OUT_QUANT_W) rs.U = max(rs.U, mag_pos(static_cast<float>(el.u)));
+                }
+            }
+        }
+    }
+    reduce_row<OUT, WARPS>(rs, red);
     float inv = 1.f;
     if (NORM) {
-        float acc = 0.f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (i0 + k * T * VEC < g.ni)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) acc += fmaf(m[k][e], m[k][e], S[k][e]);
-        acc = block_sum<WARPS>(acc, red_f);
-        inv = 1.0f / sqrtf(acc / static_cast<float>(g.ni) + g.eps);
+        inv = 1.0f / sqrtf(rs.sum / static_cast<float>(g.ni) + g.eps);
         if (i0 == 0 && g.inv) g.inv[row] = inv;
     }
     if (OUT == OUT_F32) {
@@ -258,35 +279,13 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) row_kernel(cons
         }
         return;
     }
-    unsigned P = 0, Tm = 0, U = 0;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int j = i0 + k * T * VEC;
-        if (j < g.ni) {
-            float w[VEC] = {}, sw[VEC] = {};
-            if (OUT == OUT_INT8) {
-                ld<VEC>(g.w + j, w);
-                ld<VEC>(g.Sw + j, sw);
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const Elem<OUT> el(m[k][e], S[k][e], w[e], sw[e]);
-                P = max(P, mag(static_cast<float>(el.p)));
-                Tm = max(Tm, mag_pos(static_cast<float>(el.t)));
-                if (OUT == OUT_QUANT_W) U = max(U, mag_pos(static_cast<float>(el.u)));
-            }
-        }
-    }
-    P = block_max<WARPS>(P, red_u[0]);
-    Tm = block_max<WARPS>(Tm, red_u[1]);
-    if (OUT == OUT_QUANT_W) U = block_max<WARPS>(U, red_u[2]);
-    const RowScales r = row_scales<OUT>(P, Tm, U, inv);
+    const RowScales r = row_scales<OUT>(rs.P, rs.T, rs.U, inv);
     if (i0 == 0) {
         g.scales[row] = r.sm;
         g.scales[g.rows + row] = r.s2;
         g.scales[2 * g.rows + row] = r.sS;
     }
-    const bool bad = P >= kInfBits || Tm >= kInfBits || U >= kInfBits;
+    const bool bad = rs.P >= kInfBits || rs.T >= kInfBits || rs.U >= kInfBits;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int j = i0 + k * T * VEC;
@@ -316,29 +315,34 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) row_kernel(cons
 template <int OUT>
 __global__ void __launch_bounds__(512) long_row_kernel(const NormArgs g) {
     constexpr int WARPS = 16;
-    __shared__ float red_f[WARPS];
-    __shared__ unsigned red_u[3][WARPS];
+    __shared__ RowStats red[WARPS];
     constexpr bool NORM = OUT == OUT_F32 || OUT == OUT_INT8;
     const int64_t row = blockIdx.x;
     const int64_t base = row * g.ni;
     const bool add = NORM && g.rm;
     const float* hm = (add ? g.hm : g.am) + base;
     const float* hS = (add ? g.hS : g.aS) + base;
+    RowStats rs{0.f, 0u, 0u, 0u};
+    for (int j = threadIdx.x; j < g.ni; j += blockDim.x) {
+        float x = g.am[base + j], y = g.aS[base + j];
+        if (add) {
+            x += g.rm[base + j];
+            y += g.rS[base + j];
+            g.hm[base + j] = x;
+            g.hS[base + j] = y;
+        }
+        if (NORM) rs.sum += fmaf(x, x, y);
+        if (OUT != OUT_F32) {
+            const Elem<OUT> el(x, y, OUT == OUT_INT8 ? g.w[j] : 0.f, OUT == OUT_INT8 ? g.Sw[j] : 0.f);
+            rs.P = max(rs.P, mag(static_cast<float>(el.p)));
+            rs.T = max(rs.T, mag_pos(static_cast<float>(el.t)));
+            if (OUT == OUT_QUANT_W) rs.U = max(rs.U, mag_pos(static_cast<float>(el.u)));
+        }
+    }
+    reduce_row<OUT, WARPS>(rs, red);
     float inv = 1.f;
     if (NORM) {
-        float acc = 0.f;
-        for (int j = threadIdx.x; j < g.ni; j += blockDim.x) {
-            float x = g.am[base + j], y = g.aS[base + j];
-            if (add) {
-                x += g.rm[base + j];
-                y += g.rS[base + j];
-                g.hm[base + j] = x;
-                g.hS[base + j] = y;
-            }
-            acc += fmaf(x, x, y);
-        }
-        acc = block_sum<WARPS>(acc, red_f);
-        inv = 1.0f / sqrtf(acc / static_cast<float>(g.ni) + g.eps);
+        inv = 1.0f / sqrtf(rs.sum / static_cast<float>(g.ni) + g.eps);
         if (threadIdx.x == 0 && g.inv) g.inv[row] = inv;
     }
     // every thread reads back the elements that it wrote itself
@@ -350,24 +354,13 @@ __global__ void __launch_bounds__(512) long_row_kernel(const NormArgs g) {
         }
         return;
     }
-    unsigned P = 0, Tm = 0, U = 0;
-    for (int j = threadIdx.x; j < g.ni; j += blockDim.x) {
-        const Elem<OUT> el(hm[j], hS[j], OUT == OUT_INT8 ? g.w[j] : 0.f,
-                           OUT == OUT_INT8 ? g.Sw[j] : 0.f);
-        P = max(P, mag(static_cast<float>(el.p)));
-        Tm = max(Tm, mag_pos(static_cast<float>(el.t)));
-        if (OUT == OUT_QUANT_W) U = max(U, mag_pos(static_cast<float>(el.u)));
-    }
-    P = block_max<WARPS>(P, red_u[0]);
-    Tm = block_max<WARPS>(Tm, red_u[1]);
-    U = block_max<WARPS>(U, red_u[2]);
-    const RowScales r = row_scales<OUT>(P, Tm, U, inv);
+    const RowScales r = row_scales<OUT>(rs.P, rs.T, rs.U, inv);
     if (threadIdx.x == 0) {
         g.scales[row] = r.sm;
         g.scales[g.rows + row] = r.s2;
         g.scales[2 * g.rows + row] = r.sS;
     }
-    const bool bad = P >= kInfBits || Tm >= kInfBits || U >= kInfBits;
+    const bool bad = rs.P >= kInfBits || rs.T >= kInfBits || rs.U >= kInfBits;
     for (int j = threadIdx.x; j < g.ni; j += blockDim.x) {
         const Elem<OUT> el(hm[j], hS[j], OUT == OUT_INT8 ? g.w[j] : 0.f,
                            OUT == OUT_INT8 ? g.Sw[j] : 0.f);
@@ -394,7 +387,9 @@ int launch_width(const NormArgs& g, cudaStream_t st, const char* what) {
     const int vecs = (g.ni + VEC - 1) / VEC;
     if (vecs <= 64) return launch_row<OUT, VEC, 1, 2>(g, st, what);
     if (vecs <= 128) return launch_row<OUT, VEC, 1, 4>(g, st, what);
+    if (vecs <= 256) return launch_row<OUT, VEC, 2, 4>(g, st, what);
     if (vecs <= 512) return launch_row<OUT, VEC, 4, 4>(g, st, what);
+    if (vecs <= 1024) return launch_row<OUT, VEC, 8, 4>(g, st, what);
     if (vecs <= 2048) return launch_row<OUT, VEC, 16, 4>(g, st, what);
     TAGI_REQUIRE(g.rows <= INT32_MAX, TAGI_E_UNSUPPORTED, "%s: too many rows", what);
     long_row_kernel<OUT><<<static_cast<unsigned>(g.rows), 512, 0, st>>>(g);
@@ -419,41 +414,43 @@ int launch_norm(const NormArgs& g, cudaStream_t st, const char* what) {
     return launch_width<OUT, 1>(g, st, what);
 }
 
-// code * scale, VEC codes of one of the three operands (blockIdx.y) per thread.
+// code * scale of one of the three operands (blockIdx.y), VEC codes per thread; the
+// block's y rows at a time.
 template <int VEC>
 __global__ void values_kernel(const NormArgs g, float* vm, float* v2, float* vS) {
     const int which = blockIdx.y;
-    const int per = g.ni / VEC;
-    const int64_t total = g.rows * per;
     const uint8_t* q = which == 0 ? reinterpret_cast<const uint8_t*>(g.qm)
                                   : (which == 1 ? g.q2 : g.qS);
     float* v = which == 0 ? vm : (which == 1 ? v2 : vS);
     const float* sc = g.scales + which * g.rows;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t r = i / per;
-        const int j = static_cast<int>(i - r * per) * VEC;
+    for (int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y; r < g.rows;
+         r += static_cast<int64_t>(gridDim.x) * blockDim.y) {
         const float s = sc[r];
-        const uint8_t* p = q + r * g.ldq + j;
-        uint32_t x = VEC == 4 ? *reinterpret_cast<const uint32_t*>(p) : *p;
-        float out[VEC];
+#pragma unroll 4
+        for (int j = threadIdx.x * VEC; j < g.ni; j += blockDim.x * VEC) {
+            const uint8_t* p = q + r * g.ldq + j;
+            const uint32_t x = VEC == 4 ? *reinterpret_cast<const uint32_t*>(p) : *p;
+            float out[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint32_t b = (x >> (8 * e)) & 255u;
-            out[e] = s * (which == 0 ? static_cast<float>(static_cast<int8_t>(b))
-                                     : static_cast<float>(b));
+            for (int e = 0; e < VEC; ++e) {
+                const uint32_t b = (x >> (8 * e)) & 255u;
+                out[e] = s * (which == 0 ? static_cast<float>(static_cast<int8_t>(b))
+                                         : static_cast<float>(b));
+            }
+            st<VEC>(v + r * g.ni + j, out);
         }
-        st<VEC>(v + r * g.ni + j, out);
     }
 }
 
 // ---- backward -------------------------------------------------------------------
 //   d_m = r_m + (inv w) dz_m,  d_S = r_S + (inv w)^2 dz_S
 //   sums over rows: g_m = sum inv h dz_m,  g_S = sum (inv h)^2 dz_S
-// Both are formed in one pass: block (slice, columns) walks its rows with its
-// columns' sums in registers and leaves them in the workspace; a second launch adds
-// the slices in order and applies them.
-constexpr int kBackThreads = 128;
+// Both are formed in one pass: block (slice, columns) walks its rows with its columns'
+// sums in registers, kBackThreads / x rows at a time (x threads along the columns), adds
+// the groups' sums in order and leaves them in the workspace; a second launch adds the
+// slices in order and applies them.
+constexpr int kBackThreads = 512;
+constexpr int kBackCols = 128;  // threads along the columns, at most
 
 struct BackArgs {
     const float* dm;
@@ -472,47 +469,61 @@ struct BackArgs {
 
 template <int VEC>
 __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackArgs g) {
+    __shared__ double red[2][kBackThreads * VEC];
     launch_dependents();
-    const int j = (blockIdx.y * kBackThreads + threadIdx.x) * VEC;
-    if (j >= g.ni) return;
+    const int j = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    const int groups = blockDim.y, grp = threadIdx.y;
     const int64_t r0 = static_cast<int64_t>(blockIdx.x) * g.slice_rows;
     const int64_t r1 = r0 + g.slice_rows < g.rows ? r0 + g.slice_rows : g.rows;
-    float w[VEC];
-    ld<VEC>(g.w + j, w);
     double sm[VEC], sS[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sm[e] = sS[e] = 0.0;
+    if (j < g.ni) {
+        float w[VEC];
+        ld<VEC>(g.w + j, w);
 #pragma unroll 2
-    for (int64_t r = r0; r < r1; ++r) {
-        const int64_t o = r * g.ni + j;
-        const float inv = g.inv[r];
-        float dm[VEC], dS[VEC], h[VEC], xm[VEC], xS[VEC];
-        ld<VEC>(g.dm + o, dm);
-        ld<VEC>(g.dS + o, dS);
-        ld<VEC>(g.h + o, h);
-        if (g.rm) {
-            ld<VEC>(g.rm + o, xm);
-            ld<VEC>(g.rS + o, xS);
-        } else {
+        for (int64_t r = r0 + grp; r < r1; r += groups) {
+            const int64_t o = r * g.ni + j;
+            const float inv = g.inv[r];
+            float dm[VEC], dS[VEC], h[VEC], xm[VEC], xS[VEC];
+            ld<VEC>(g.dm + o, dm);
+            ld<VEC>(g.dS + o, dS);
+            ld<VEC>(g.h + o, h);
+            if (g.rm) {
+                ld<VEC>(g.rm + o, xm);
+                ld<VEC>(g.rS + o, xS);
+            } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) xm[e] = xS[e] = 0.f;
-        }
+                for (int e = 0; e < VEC; ++e) xm[e] = xS[e] = 0.f;
+            }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float t = inv * w[e], x = inv * h[e];
-            xm[e] += t * dm[e];
-            xS[e] += t * t * dS[e];
-            sm[e] += static_cast<double>(x * dm[e]);
-            sS[e] += static_cast<double>(x * x * dS[e]);
+            for (int e = 0; e < VEC; ++e) {
+                const float t = inv * w[e], x = inv * h[e];
+                xm[e] += t * dm[e];
+                xS[e] += t * t * dS[e];
+                sm[e] += static_cast<double>(x * dm[e]);
+                sS[e] += static_cast<double>(x * x * dS[e]);
+            }
+            st<VEC>(g.om + o, xm);
+            st<VEC>(g.oS + o, xS);
         }
-        st<VEC>(g.om + o, xm);
-        st<VEC>(g.oS + o, xS);
     }
-    double* p = g.part + static_cast<int64_t>(blockIdx.x) * 2 * g.ni + j;
+    const int at = (grp * blockDim.x + threadIdx.x) * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        p[e] = sm[e];
-        p[g.ni + e] = sS[e];
+        red[0][at + e] = sm[e];
+        red[1][at + e] = sS[e];
+    }
+    __syncthreads();
+    // a thread per column and sum
+    const int cols = blockDim.x * VEC;
+    for (int i = grp * blockDim.x + threadIdx.x; i < 2 * cols; i += kBackThreads) {
+        const int which = i / cols, c = i - which * cols;
+        const int col = blockIdx.y * cols + c;
+        if (col >= g.ni) continue;
+        double a = red[which][c];
+        for (int k = 1; k < groups; ++k) a += red[which][k * cols + c];
+        g.part[(static_cast<int64_t>(blockIdx.x) * 2 + which) * g.ni + col] = a;
     }
 }
 
@@ -565,11 +576,20 @@ __global__ void __launch_bounds__(256) back_finish_kernel(const double* part, in
     Sw[j] = v;
 }
 
-// Slices of rows: enough blocks to fill the SMs several times, 8 rows or more each.
-int slices_of(int64_t rows, int64_t ni) {
-    const int64_t cols = (ni + 4 * kBackThreads - 1) / (4 * kBackThreads);
-    int64_t s = (kNumSMs * 4 + cols - 1) / cols;
-    const int64_t most = (rows + 7) / 8;
+// Threads along the columns of `vecs` vectors, and slices of rows: three blocks per SM
+// (what their registers allow), 2 rows or more for each of a block's groups.
+int back_x(int64_t vecs) {
+    int x = 32;
+    while (x < kBackCols && x < vecs) x *= 2;
+    return x;
+}
+int slices_of(int64_t rows, int64_t ni, int vec) {
+    const int64_t vecs = (ni + vec - 1) / vec;
+    const int x = back_x(vecs);
+    const int64_t cols = (vecs + x - 1) / x;
+    int64_t s = (kNumSMs * 2 + cols - 1) / cols;
+    const int64_t per = 2 * (kBackThreads / x);
+    const int64_t most = (rows + per - 1) / per;
     if (s > most) s = most;
     return static_cast<int>(s < 1 ? 1 : s);
 }
@@ -658,19 +678,23 @@ extern "C" int tagi_int8_values(const int8_t* q_m, const uint8_t* q_2, const uin
     for (const void* p : {static_cast<const void*>(q_m), static_cast<const void*>(q_2),
                           static_cast<const void*>(q_S)})
         bits |= reinterpret_cast<uintptr_t>(p) * 4;
-    if (ni % 4 == 0 && (bits & 15) == 0) {
-        const dim3 grid(grid_1d(rows * (ni / 4), 256), 3);
-        values_kernel<4><<<grid, 256, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
-    } else {
-        const dim3 grid(grid_1d(rows * ni, 256), 3);
-        values_kernel<1><<<grid, 256, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
-    }
+    const bool v4 = ni % 4 == 0 && (bits & 15) == 0;
+    const int64_t vecs = v4 ? ni / 4 : ni;
+    int x = 32;
+    while (x < 256 && x < vecs) x *= 2;
+    const dim3 block(x, 256 / x), grid(grid_1d(rows, 256 / x, kNumSMs * 32), 3);
+    if (v4)
+        values_kernel<4><<<grid, block, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
+    else
+        values_kernel<1><<<grid, block, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
     return check_launch(what);
 }
 
 extern "C" size_t tagi_add_rmsnorm_backward_workspace_size(int64_t rows, int64_t ni) {
     if (rows < 0 || ni < 1) return 0;
-    return static_cast<size_t>(slices_of(rows, ni)) * 2 * static_cast<size_t>(ni) * sizeof(double);
+    // the larger of both vector widths: alignment is not known here
+    const int a = slices_of(rows, ni, 4), b = slices_of(rows, ni, 1);
+    return static_cast<size_t>(a > b ? a : b) * 2 * static_cast<size_t>(ni) * sizeof(double);
 }
 
 extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, const float* hm,
@@ -695,14 +719,10 @@ extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, con
     TAGI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, TAGI_E_ALIGNMENT,
                  "%s: workspace not 16-byte aligned", what);
     cudaStream_t st = as_stream(stream);
-    const int slices = slices_of(rows, ni);
     BackArgs g{};
     g.dm = dmz; g.dS = dSz; g.h = hm; g.inv = inv_rms; g.w = mw; g.rm = rm; g.rS = rS;
     g.om = d_m; g.oS = d_S; g.part = static_cast<double*>(workspace);
     g.rows = rows; g.ni = static_cast<int>(ni);
-    const int64_t per = (rows + slices - 1) / slices;
-    TAGI_REQUIRE(per <= INT32_MAX, TAGI_E_UNSUPPORTED, "%s: too many rows", what);
-    g.slice_rows = static_cast<int>(per < 1 ? 1 : per);
     uintptr_t bits = 0;
     for (const void* p : {static_cast<const void*>(dmz), static_cast<const void*>(dSz),
                           static_cast<const void*>(hm), static_cast<const void*>(rm),
@@ -710,13 +730,18 @@ extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, con
                           static_cast<const void*>(d_m), static_cast<const void*>(d_S)})
         bits |= reinterpret_cast<uintptr_t>(p);
     const bool v4 = ni % 4 == 0 && (bits & 15) == 0;
-    const int cols = kBackThreads * (v4 ? 4 : 1);
-    const dim3 grid(slices, static_cast<unsigned>((ni + cols - 1) / cols));
-    TAGI_REQUIRE(grid.y <= 65535, TAGI_E_UNSUPPORTED, "%s: too many columns", what);
+    const int slices = slices_of(rows, ni, v4 ? 4 : 1);
+    const int64_t per = (rows + slices - 1) / slices;
+    TAGI_REQUIRE(per <= INT32_MAX, TAGI_E_UNSUPPORTED, "%s: too many rows", what);
+    g.slice_rows = static_cast<int>(per < 1 ? 1 : per);
+    const int64_t vecs = v4 ? ni / 4 : ni;
+    const int x = back_x(vecs);
+    const dim3 grid(slices, static_cast<unsigned>((vecs + x - 1) / x)), block(x, kBackThreads / x);
+    TAGI_REQUIRE((vecs + x - 1) / x <= 65535, TAGI_E_UNSUPPORTED, "%s: too many columns", what);
     if (v4)
-        back_kernel<4><<<grid, kBackThreads, 0, st>>>(g);
+        back_kernel<4><<<grid, block, 0, st>>>(g);
     else
-        back_kernel<1><<<grid, kBackThreads, 0, st>>>(g);
+        back_kernel<1><<<grid, block, 0, st>>>(g);
     const int rc = check_launch(what);
     if (rc) return rc;
     launch_early(back_finish_kernel, dim3(static_cast<unsigned>((ni + 7) / 8)), dim3(256), st,
