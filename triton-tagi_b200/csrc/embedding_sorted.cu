@@ -204,13 +204,15 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
         }
         cluster.sync();
         if (threadIdx.x < kBins) {
+            int c[kSortCluster];  // all remote loads in flight together
+#pragma unroll
+            for (int r = 0; r < kSortCluster; ++r)
+                c[r] = r < ctas ? *cluster.map_shared_rank(&total[threadIdx.x], r) : 0;
             int before = 0, all = 0;
 #pragma unroll
             for (int r = 0; r < kSortCluster; ++r) {
-                if (r >= ctas) break;
-                const int c = *cluster.map_shared_rank(&total[threadIdx.x], r);
-                if (r < rank) before += c;
-                all += c;
+                if (r < rank) before += c[r];
+                all += c[r];
             }
             int incl = all;  // inclusive scan over the digits
 #pragma unroll
@@ -469,24 +471,20 @@ template <int VEC, int MODE>
 __global__ void __launch_bounds__(32 * kGroups) join_kernel(const GradArgs a) {
     __shared__ double sum[2][kGroups][32 * VEC];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int cols = (a.D + 32 * VEC - 1) / (32 * VEC);
+    const int j = (blockIdx.y * 32 + lane) * VEC;
     wait_for_primary();  // the partials and the list of segments
     const int shorts = a.listed[0], longs = a.listed[1];
-    for (int64_t it = static_cast<int64_t>(blockIdx.x) * kGroups + g;
-         it < static_cast<int64_t>(shorts) * cols; it += static_cast<int64_t>(gridDim.x) * kGroups) {
-        const int j = (static_cast<int>(it % cols) * 32 + lane) * VEC;
-        if (j >= a.D) continue;
-        const int4 c = a.list[it / cols];
+    for (int it = blockIdx.x * kGroups + g; it < shorts && j < a.D; it += gridDim.x * kGroups) {
+        const int4 c = a.list[it];
         const int64_t o = static_cast<int64_t>(c.z) * a.D + j;
         double m[VEC] = {}, S[VEC] = {};
         float mean[VEC], w[VEC];
-        add_partials<VEC>(a, c.x, c.x, 1, c.y, j, m, S);
         params<VEC, MODE>(a, o, mean, w);
+        add_partials<VEC>(a, c.x, c.x, 1, c.y, j, m, S);
         finish<VEC, MODE>(a, o, m, S, mean, w);
     }
-    for (int64_t it = blockIdx.x; it < static_cast<int64_t>(longs) * cols; it += gridDim.x) {
-        const int4 c = a.list[a.chunks - 1 - it / cols];
-        const int j = (static_cast<int>(it % cols) * 32 + lane) * VEC;
+    for (int it = blockIdx.x; it < longs; it += gridDim.x) {
+        const int4 c = a.list[a.chunks - 1 - it];
         const int64_t o = static_cast<int64_t>(c.z) * a.D + j;
         double m[VEC] = {}, S[VEC] = {};
         if (j < a.D) add_partials<VEC>(a, c.x, c.x + g, kGroups, c.y, j, m, S);
@@ -574,8 +572,10 @@ int launch_grad(GradArgs a, cudaStream_t st, const char* what) {
     launch_early(reduce_kernel<VEC, MODE>, grid, dim3(threads), st, a);
     const int rc = check_launch(what);
     if (rc || a.chunks <= 1) return rc;
-    const int64_t items = (static_cast<int64_t>(a.chunks - 1) * ((vecs + 31) / 32) + kGroups - 1) / kGroups;
-    launch_early(join_kernel<VEC, MODE>, dim3(grid_1d(items, 1, kNumSMs * 8)), dim3(32 * kGroups), st,
+    const int cols = (vecs + 31) / 32;
+    const unsigned most = (a.chunks + kGroups - 2) / kGroups;  // a warp per segment
+    const unsigned fill = (kNumSMs * 8 + cols - 1) / cols;
+    launch_early(join_kernel<VEC, MODE>, dim3(most < fill ? most : fill, cols), dim3(32 * kGroups), st,
                  a);
     return check_launch(what);
 }

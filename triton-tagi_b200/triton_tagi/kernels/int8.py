@@ -37,12 +37,12 @@ class Int8Moments(NamedTuple):
     def values(self) -> tuple[Tensor, Tensor, Tensor]:
         """What the codes stand for: three float32 ``(rows, width)`` tensors."""
         dev = check_f32(self.scales)
-        q = _checked(self, dev)
-        rows, width = q.q_m.shape
-        out = [q.scales.new_empty((rows, width)) for _ in range(3)]
-        call_on(dev, "tagi_int8_values", *_pointers(q), *(t.data_ptr() for t in out), rows,
-                width)
-        return tuple(out)
+        pointers, rows, width, _hold = _checked(self, dev)
+        new = self.scales.new_empty
+        v_m, v_2, v_S = new((rows, width)), new((rows, width)), new((rows, width))
+        call_on(dev, "tagi_int8_values", *pointers, v_m.data_ptr(), v_2.data_ptr(), v_S.data_ptr(),
+                rows, width)
+        return v_m, v_2, v_S
 
 
 def empty_codes(rows: int, width: int, like: Tensor) -> Int8Moments:
@@ -56,35 +56,45 @@ def empty_codes(rows: int, width: int, like: Tensor) -> Int8Moments:
                        like.new_empty((3, rows), dtype=torch.float32))
 
 
-def _ld(t: Tensor) -> int:
-    """Bytes between rows of codes (of one row: any multiple of 16 that holds it)."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
-
-
-def _checked(q: Int8Moments, dev: int) -> Int8Moments:
-    """``q`` with the layout the kernels read: unit column stride, one row stride, rows
-    on 16-byte boundaries (copied where it differs)."""
+def _checked(q: Int8Moments, dev: int) -> tuple:
+    """(pointers and row stride, rows, width, codes) of ``q`` in the layout that the
+    kernels read: unit column stride, one row stride, rows on 16-byte boundaries; the
+    codes are copied where theirs differs."""
     q_m, q_2, q_S, scales = q
     check_on(dev, q_m, q_2, q_S)
-    if q_m.dtype != torch.int8 or q_2.dtype != torch.uint8 or q_S.dtype != torch.uint8:
+    if q_m.dtype is not torch.int8 or q_2.dtype is not torch.uint8 or q_S.dtype is not torch.uint8:
         raise ValueError(f"codes must be int8, uint8, uint8, got {q_m.dtype}, {q_2.dtype}, "
                          f"{q_S.dtype}")
-    if q_m.dim() != 2 or q_2.shape != q_m.shape or q_S.shape != q_m.shape \
-            or tuple(scales.shape) != (3, q_m.shape[0]):
-        raise ValueError(f"codes {tuple(q_m.shape)}, {tuple(q_2.shape)}, {tuple(q_S.shape)} and "
+    shape = q_m.shape
+    if len(shape) != 2 or q_2.shape != shape or q_S.shape != shape \
+            or scales.shape != (3, shape[0]):
+        raise ValueError(f"codes {tuple(shape)}, {tuple(q_2.shape)}, {tuple(q_S.shape)} and "
                          f"scales {tuple(scales.shape)} do not belong together")
-    ld = _ld(q_m)
-    if any(t.stride(1) != 1 or _ld(t) != ld or ld < t.shape[1] or (ld | t.data_ptr()) & 15
-           for t in (q_m, q_2, q_S)):
-        new = empty_codes(*q_m.shape, scales)
-        for a, b in zip(new[:3], (q_m, q_2, q_S)):
-            a.copy_(b)
-        q = Int8Moments(*new[:3], scales)
-    return q if scales.is_contiguous() else q._replace(scales=scales.contiguous())
+    rows, width = shape
+    stride = q_m.stride()
+    ld = stride[0]
+    if rows <= 1:  # the stride of a single row says nothing
+        ld = (width + 15) // 16 * 16
+        same = q_m.stride(1) == q_2.stride(1) == q_S.stride(1) == 1
+    else:
+        same = stride[1] == 1 and q_2.stride() == stride and q_S.stride() == stride
+    if not same or ld < width \
+            or (ld | q_m.data_ptr() | q_2.data_ptr() | q_S.data_ptr()) & 15:
+        new = empty_codes(rows, width, scales)
+        new.q_m.copy_(q_m)
+        new.q_2.copy_(q_2)
+        new.q_S.copy_(q_S)
+        q_m, q_2, q_S = new[:3]
+        ld = (width + 15) // 16 * 16
+    scales = scales.contiguous()
+    return ((q_m.data_ptr(), q_2.data_ptr(), q_S.data_ptr(), scales.data_ptr(), ld), rows, width,
+            (q_m, q_2, q_S, scales))
 
 
-def _pointers(q: Int8Moments) -> tuple:
-    return (q.q_m.data_ptr(), q.q_2.data_ptr(), q.q_S.data_ptr(), q.scales.data_ptr(), _ld(q.q_m))
+def _pointers(q: Int8Moments, width: int) -> tuple:
+    """Pointers and row stride of codes from ``empty_codes``."""
+    return (q.q_m.data_ptr(), q.q_2.data_ptr(), q.q_S.data_ptr(), q.scales.data_ptr(),
+            (width + 15) // 16 * 16)
 
 
 def _quantize(m: Tensor, S: Tensor, weights: bool) -> Int8Moments:
@@ -96,7 +106,7 @@ def _quantize(m: Tensor, S: Tensor, weights: bool) -> Int8Moments:
     m, S = m.reshape(-1, width).contiguous(), S.reshape(-1, width).contiguous()
     q = empty_codes(m.shape[0], width, m)
     call_on(dev, "tagi_quantize_moments", m.data_ptr(), S.data_ptr(), 1 if weights else 0,
-            *_pointers(q), m.shape[0], width)
+            *_pointers(q, width), m.shape[0], width)
     return q
 
 
@@ -118,17 +128,16 @@ def int8_moments_matmul(x: Int8Moments, w: Int8Moments, mb: Tensor | None = None
     """(mz, Sz), each ``(M, N)``: the moments of tokens ``x`` (M, K) through weights
     ``w`` (N, K) plus the biases (N values each, or None)."""
     dev = check_f32(x.scales, w.scales, mb, Sb)
-    x, w = _checked(x, dev), _checked(w, dev)
-    M, K = x.q_m.shape
-    N = w.q_m.shape[0]
-    if w.q_m.shape[1] != K:
-        raise ValueError(f"Reduction dims disagree: x has {K}, w has {w.q_m.shape[1]}")
+    px, M, K, _hold_x = _checked(x, dev)
+    pw, N, Kw, _hold_w = _checked(w, dev)
+    if Kw != K:
+        raise ValueError(f"Reduction dims disagree: x has {K}, w has {Kw}")
     if mb is not None and mb.numel() != N or Sb is not None and Sb.numel() != N:
         raise ValueError(f"biases must hold {N} values")
     mb = None if mb is None else mb.contiguous()
     Sb = None if Sb is None else Sb.contiguous()
     mz = x.scales.new_empty((M, N))
     Sz = torch.empty_like(mz)
-    call_on(dev, "tagi_int8_moment_matmul", *_pointers(x), *_pointers(w), ptr(mb), ptr(Sb),
+    call_on(dev, "tagi_int8_moment_matmul", *px, *pw, ptr(mb), ptr(Sb),
             mz.data_ptr(), Sz.data_ptr(), M, N, K)
     return mz, Sz

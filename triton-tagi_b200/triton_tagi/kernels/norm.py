@@ -25,8 +25,11 @@ def _rows(name: str, mw: Tensor, Sw: Tensor | None, *ts: Tensor | None) -> tuple
     if width < 1 or Sw is not None and Sw.numel() != width:
         raise ValueError(f"{name}: scale parameters of {mw.numel()} and "
                          f"{'no' if Sw is None else Sw.numel()} values")
+    shape = first.shape
+    if not shape or shape[-1] != width:
+        raise ValueError(f"{name}: rows of {width} do not fit shape {tuple(shape)}")
     for t in ts:
-        if t is not None and (t.dim() < 1 or t.shape[-1] != width or t.shape != first.shape):
+        if t is not None and t.shape != shape:
             raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit {tuple(first.shape)} "
                              f"with rows of {width}")
     return dev, first.numel() // width, width
@@ -67,7 +70,7 @@ def add_rmsnorm_int8(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | Non
     hm, hS = (ma, Sa) if mr is None else (torch.empty_like(ma), torch.empty_like(Sa))
     q = empty_codes(rows, width, ma)
     call_on(dev, "tagi_add_rmsnorm_int8", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
-            mw.data_ptr(), Sw.data_ptr(), hm.data_ptr(), hS.data_ptr(), *_pointers(q), rows,
+            mw.data_ptr(), Sw.data_ptr(), hm.data_ptr(), hS.data_ptr(), *_pointers(q, width), rows,
             width, eps)
     return hm, hS, q
 
