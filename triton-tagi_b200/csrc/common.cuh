@@ -151,17 +151,28 @@ inline unsigned grid_1d(int64_t n, int threads, int64_t max_blocks = 148 * 16) {
 // launch itself is hidden. It calls wait_for_primary() before it touches anything that
 // the one before it writes or reads; that returns when that kernel has ended and its
 // writes are visible.
+struct EarlyLaunch {
+    dim3 grid, block;
+    cudaStream_t stream;
+    size_t smem = 0;
+    dim3 cluster = dim3(1, 1, 1);
+};
 template <typename... P, typename... A>
-inline void launch_early(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
+inline void launch_early(void (*kernel)(P...), const EarlyLaunch& l, const A&... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cfg.gridDim = l.grid;
+    cfg.blockDim = l.block;
+    cfg.stream = l.stream;
+    cfg.dynamicSmemBytes = l.smem;
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = l.cluster.x;
+    at[1].val.clusterDim.y = l.cluster.y;
+    at[1].val.clusterDim.z = l.cluster.z;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = l.cluster.x * l.cluster.y * l.cluster.z > 1 ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 __device__ __forceinline__ void launch_dependents() {

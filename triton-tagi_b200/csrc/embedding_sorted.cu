@@ -80,8 +80,10 @@ __device__ __forceinline__ void stv(float* p, const float (&v)[VEC]) {
 template <int VEC, int IDT>
 __global__ void lookup_kernel(const void* ids, const float* mw, const float* Sw, float* mz,
                               float* Sz, int64_t n, int V, int D, int64_t pad, float s, float s2) {
+    launch_dependents();
     const int per = D / VEC;
     const int64_t total = n * per;
+    wait_for_primary();
     for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t t = i / per;
@@ -146,6 +148,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a)
     const int hi = static_cast<int>(first + per < a.n ? first + per : a.n);
     const int mask = (1 << a.bits) - 1;
     const bool single = per <= 32 * kItems;
+    wait_for_primary();
     if (rank == 0 && threadIdx.x < 2) a.listed[threadIdx.x] = 0;
 
     for (int pass = 0; pass < a.passes; ++pass) {
@@ -543,17 +546,7 @@ int launch_sort(const SortArgs& a, cudaStream_t st, const char* what) {
         set_error("%s: clusters of %d refused (%s)", what, kSortCluster, cudaGetErrorString(e));
         return TAGI_E_LAUNCH;
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kSortThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ctas;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, sort_kernel<IDT>, a);
+    launch_early(sort_kernel<IDT>, {dim3(ctas), dim3(kSortThreads), st, 0, dim3(ctas)}, a);
     return check_launch(what);
 }
 
@@ -569,14 +562,14 @@ int launch_grad(GradArgs a, cudaStream_t st, const char* what) {
     if (a.chunks + zero == 0) return TAGI_OK;
     TAGI_REQUIRE(a.chunks + zero <= INT32_MAX, TAGI_E_UNSUPPORTED, "%s: sizes beyond the grid", what);
     const dim3 grid(static_cast<unsigned>(a.chunks + zero), slices);
-    launch_early(reduce_kernel<VEC, MODE>, grid, dim3(threads), st, a);
+    launch_early(reduce_kernel<VEC, MODE>, {grid, dim3(threads), st}, a);
     const int rc = check_launch(what);
     if (rc || a.chunks <= 1) return rc;
     const int cols = (vecs + 31) / 32;
     const unsigned most = (a.chunks + kGroups - 2) / kGroups;  // a warp per segment
     const unsigned fill = (kNumSMs * 8 + cols - 1) / cols;
-    launch_early(join_kernel<VEC, MODE>, dim3(most < fill ? most : fill, cols), dim3(32 * kGroups), st,
-                 a);
+    launch_early(join_kernel<VEC, MODE>,
+                 {dim3(most < fill ? most : fill, cols), dim3(32 * kGroups), st}, a);
     return check_launch(what);
 }
 
@@ -607,8 +600,9 @@ extern "C" int tagi_embedding_lookup(const void* ids, int id_type, const float* 
     const float s2 = scale * scale;
     cudaStream_t st = as_stream(stream);
 #define LOOKUP(VEC, IDT)                                                                      \
-    lookup_kernel<VEC, IDT><<<grid_1d(n * (D / VEC), 256), 256, 0, st>>>(                     \
-        ids, mw, Sw, mz, Sz, n, static_cast<int>(V), static_cast<int>(D), padding_idx, scale, s2)
+    launch_early(lookup_kernel<VEC, IDT>, {dim3(grid_1d(n * (D / VEC), 256)), dim3(256), st}, \
+                 ids, mw, Sw, mz, Sz, n, static_cast<int>(V), static_cast<int>(D),            \
+                 padding_idx, scale, s2)
 #define LOOKUP_V(IDT)                 \
     if (vec == 4) LOOKUP(4, IDT);     \
     else if (vec == 2) LOOKUP(2, IDT); \

@@ -255,7 +255,7 @@ constexpr int kPairSmem = kPairStages * kPairStage + 1024;
 constexpr int kPairReaders = 16;  // epilogue warps: 4 per lane quarter, 64 columns each
 constexpr int kPairThreads = 64 + 32 * kPairReaders;
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     int8_pair_kernel(const Int8Args g, const __grid_constant__ Maps maps) {
     extern __shared__ char raw[];
     __shared__ __align__(8) uint64_t landed[kPairStages], peer_landed[kPairStages],
@@ -272,6 +272,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int tiles = ctiles * ((g.M + 255) / 256);
     const int pairs = gridDim.x / 2;
     const Abort ab{&abort_flag, map_to(smem_u32(&abort_flag), rank ^ 1)};
+    launch_dependents();
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) {
@@ -299,6 +300,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     __syncthreads();
     cluster_sync();  // both CTAs' barriers exist before any remote arrival
     tc_fence_after();
+    wait_for_primary();
     const uint32_t tmem = tmem_base;
 
     if (warp == 0) {
@@ -509,6 +511,7 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
     const int kblocks = (g.K + kBK - 1) / kBK;
     const int beg = share(3 * kblocks, rank, ctas), end = share(3 * kblocks, rank + 1, ctas);
     const Abort ab{&abort_flag, 0};
+    launch_dependents();
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < P::STAGES; ++s) {
@@ -531,6 +534,7 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base;
+    wait_for_primary();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -760,7 +764,10 @@ int launch_pair(const Int8Args& g, const Maps& maps, cudaStream_t st, const char
     const int64_t tiles = ((static_cast<int64_t>(g.M) + 255) / 256) * ((g.N + 255) / 256);
     TAGI_REQUIRE(tiles <= INT32_MAX / 2, TAGI_E_UNSUPPORTED, "%s: too many tiles", what);
     const int64_t pairs = tiles < kNumSMs / 2 ? tiles : kNumSMs / 2;
-    int8_pair_kernel<<<static_cast<unsigned>(2 * pairs), kPairThreads, kPairSmem, st>>>(g, maps);
+    launch_early(int8_pair_kernel,
+                 {dim3(static_cast<unsigned>(2 * pairs)), dim3(kPairThreads), st, kPairSmem,
+                  dim3(2)},
+                 g, maps);
     count_tc_launch();
     return check_launch(what);
 }
@@ -771,18 +778,10 @@ int launch_split(const Int8Args& g, const Maps& maps, int ctas, cudaStream_t st,
     if (const int rc = reserve_smem(int8_split_kernel<BN>, P::SMEM, what)) return rc;
     const int64_t my = (static_cast<int64_t>(g.M) + BN - 1) / BN;
     TAGI_REQUIRE(my <= 65535, TAGI_E_UNSUPPORTED, "%s: too many rows", what);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((g.N + 127) / 128, static_cast<unsigned>(my), ctas);
-    cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = P::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = cfg.gridDim.z;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, int8_split_kernel<BN>, g, maps);
+    launch_early(int8_split_kernel<BN>,
+                 {dim3((g.N + 127) / 128, static_cast<unsigned>(my), ctas), dim3(kSplitThreads), st,
+                  P::SMEM, dim3(1, 1, ctas)},
+                 g, maps);
     count_tc_launch();
     return check_launch(what);
 }

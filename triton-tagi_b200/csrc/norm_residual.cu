@@ -194,6 +194,8 @@ __device__ __forceinline__ void codes(const Elem<OUT>& e, const RowScales& r, in
 template <int OUT, int VEC, int WARPS, int NV>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) row_kernel(const NormArgs g) {
     __shared__ RowStats red[WARPS];
+    launch_dependents();
+    wait_for_primary();
     constexpr int T = 32 * WARPS;
     const int64_t row = WARPS == 1
                             ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5)
@@ -316,6 +318,8 @@ template <int OUT>
 __global__ void __launch_bounds__(512) long_row_kernel(const NormArgs g) {
     constexpr int WARPS = 16;
     __shared__ RowStats red[WARPS];
+    launch_dependents();
+    wait_for_primary();
     constexpr bool NORM = OUT == OUT_F32 || OUT == OUT_INT8;
     const int64_t row = blockIdx.x;
     const int64_t base = row * g.ni;
@@ -378,7 +382,8 @@ int launch_row(const NormArgs& g, cudaStream_t st, const char* what) {
     const int threads = WARPS == 1 ? 128 : 32 * WARPS;
     const int64_t blocks = WARPS == 1 ? (g.rows + 3) / 4 : g.rows;
     TAGI_REQUIRE(blocks <= INT32_MAX, TAGI_E_UNSUPPORTED, "%s: too many rows", what);
-    row_kernel<OUT, VEC, WARPS, NV><<<static_cast<unsigned>(blocks), threads, 0, st>>>(g);
+    launch_early(row_kernel<OUT, VEC, WARPS, NV>,
+                 {dim3(static_cast<unsigned>(blocks)), dim3(threads), st}, g);
     return check_launch(what);
 }
 
@@ -392,7 +397,7 @@ int launch_width(const NormArgs& g, cudaStream_t st, const char* what) {
     if (vecs <= 1024) return launch_row<OUT, VEC, 8, 4>(g, st, what);
     if (vecs <= 2048) return launch_row<OUT, VEC, 16, 4>(g, st, what);
     TAGI_REQUIRE(g.rows <= INT32_MAX, TAGI_E_UNSUPPORTED, "%s: too many rows", what);
-    long_row_kernel<OUT><<<static_cast<unsigned>(g.rows), 512, 0, st>>>(g);
+    launch_early(long_row_kernel<OUT>, {dim3(static_cast<unsigned>(g.rows)), dim3(512), st}, g);
     return check_launch(what);
 }
 
@@ -418,6 +423,8 @@ int launch_norm(const NormArgs& g, cudaStream_t st, const char* what) {
 // block's y rows at a time.
 template <int VEC>
 __global__ void values_kernel(const NormArgs g, float* vm, float* v2, float* vS) {
+    launch_dependents();
+    wait_for_primary();
     const int which = blockIdx.y;
     const uint8_t* q = which == 0 ? reinterpret_cast<const uint8_t*>(g.qm)
                                   : (which == 1 ? g.q2 : g.qS);
@@ -471,6 +478,7 @@ template <int VEC>
 __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackArgs g) {
     __shared__ double red[2][kBackThreads * VEC];
     launch_dependents();
+    wait_for_primary();
     const int j = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
     const int groups = blockDim.y, grp = threadIdx.y;
     const int64_t r0 = static_cast<int64_t>(blockIdx.x) * g.slice_rows;
@@ -684,9 +692,9 @@ extern "C" int tagi_int8_values(const int8_t* q_m, const uint8_t* q_2, const uin
     while (x < 256 && x < vecs) x *= 2;
     const dim3 block(x, 256 / x), grid(grid_1d(rows, 256 / x, kNumSMs * 32), 3);
     if (v4)
-        values_kernel<4><<<grid, block, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
+        launch_early(values_kernel<4>, {grid, block, as_stream(stream)}, g, v_m, v_2, v_S);
     else
-        values_kernel<1><<<grid, block, 0, as_stream(stream)>>>(g, v_m, v_2, v_S);
+        launch_early(values_kernel<1>, {grid, block, as_stream(stream)}, g, v_m, v_2, v_S);
     return check_launch(what);
 }
 
@@ -739,12 +747,12 @@ extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, con
     const dim3 grid(slices, static_cast<unsigned>((vecs + x - 1) / x)), block(x, kBackThreads / x);
     TAGI_REQUIRE((vecs + x - 1) / x <= 65535, TAGI_E_UNSUPPORTED, "%s: too many columns", what);
     if (v4)
-        back_kernel<4><<<grid, block, 0, st>>>(g);
+        launch_early(back_kernel<4>, {grid, block, st}, g);
     else
-        back_kernel<1><<<grid, block, 0, st>>>(g);
+        launch_early(back_kernel<1>, {grid, block, st}, g);
     const int rc = check_launch(what);
     if (rc) return rc;
-    launch_early(back_finish_kernel, dim3(static_cast<unsigned>((ni + 7) / 8)), dim3(256), st,
+    launch_early(back_finish_kernel, {dim3(static_cast<unsigned>((ni + 7) / 8)), dim3(256), st},
                  static_cast<const double*>(g.part), slices, g.ni, mode, sums, mw, Sw, d_mw, d_Sw,
                  cap_factor);
     return check_launch(what);
