@@ -585,3 +585,212 @@ def test_two_streams_at_once():
     for out, ref in got:
         for x, y in zip(out, ref):
             assert torch.equal(x, y)
+
+
+# -- through the layers -----------------------------------------------------------------
+
+
+def small_net(sorted_grad, seed=0, V=50, E=32, S=12, **kw):
+    import triton_tagi as tt
+
+    torch.manual_seed(seed)
+    d = dict(device=DEV)
+    return tt.Sequential([tt.Embedding(V, E, scale=0.25, sorted_grad=sorted_grad, **d, **kw),
+                          tt.PositionalEncoding(E, **d), tt.MultiheadAttentionV2(E, 4, S, **d),
+                          tt.RMSNorm(E, **d), tt.Linear(E, 64, **d), tt.ReLU(),
+                          tt.Linear(64, V, **d)], device=DEV)
+
+
+def small_batch(V=50, S=12, B=8):
+    g = gen(11)
+    x = torch.randint(0, V, (B, S), device=DEV, generator=g)
+    y = torch.nn.functional.one_hot(x.flip(1), V).float()
+    return x.float(), y
+
+
+@pytest.mark.parametrize("fuse", [True, False])
+def test_a_sorted_gradient_trains_as_the_scan_does(fuse):
+    """The same step with either gradient: rows sum at most 96 deltas, so the sums differ by
+    at most 2 x 96 roundings, and the updates by that share of a capped step."""
+    x, y = small_batch()
+    nets = [small_net(s) for s in (False, True)]
+    for net in nets:
+        net.fuse_update = fuse
+    for a, b in zip(nets[0].leaves(), nets[1].leaves()):
+        for n in ("mw", "Sw"):
+            getattr(b, n).copy_(getattr(a, n))
+    before = nets[0].layers[0].mw.clone(), nets[0].layers[0].Sw.clone()
+    outs = [net.step(x, y, 0.05) for net in nets]
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    a, b = nets[0].layers[0], nets[1].layers[0]
+    named = torch.zeros(50, dtype=torch.bool, device=DEV)
+    named[x.long()] = True
+    assert not torch.equal(a.mw[named], before[0][named])
+    assert torch.equal(b.mw[~named], before[0][~named]) and torch.equal(b.Sw[~named], before[1][~named])
+    bound = before[1].clamp_min(1e-10).sqrt() / 2.0  # no step is longer
+    for got, ref, old in ((b.mw, a.mw, before[0]), (b.Sw, a.Sw, before[1])):
+        # a step is a product with Sw and Sw^2 of sums whose terms may cancel: compare
+        # with the sums' absolute size through the bound, generously
+        assert ((got - ref).abs() <= 1e-3 * bound + 4 * U * old.abs()).all()
+
+
+def test_a_scaled_embedding_equals_a_scaled_table():
+    """Looking up s w is looking up w' = s w: forward outputs match those of a scaled table,
+    and the deltas are Sw s sum(dm), Sw^2 s^2 sum(dS)."""
+    import triton_tagi as tt
+
+    emb = tt.Embedding(40, 24, device=DEV, out_scale=3.0, padding_idx=2)
+    g = gen(12)
+    ids = torch.randint(0, 40, (6, 5), device=DEV, generator=g).float()
+    mz, Sz = emb.forward(ids, torch.zeros_like(ids))
+    i, keep = ids.long(), (ids != 2).unsqueeze(-1)
+    assert torch.equal(mz, torch.where(keep, emb.mw[i] * 3.0, 0.0))
+    assert torch.equal(Sz, torch.where(keep, emb.Sw[i] * 9.0, 0.0))
+    dm, dS = randn(g, 6, 5, 24), -rand(g, 6, 5, 24)
+    emb.backward(dm, dS)
+    r_m, r_S, t_m, t_S = plain_sums(ids.view(-1), dm.view(-1, 24), dS.view(-1, 24), 40, 2, 3.0)
+    W = emb.Sw.double()
+    within(emb.delta_mw, W * r_m, 35 * U * W * t_m, "delta_mw")
+    within(emb.delta_Sw, W * W * r_S, 36 * U * W * W * t_S, "delta_Sw")
+
+
+@pytest.mark.parametrize("mode", ["deltas", "update", "sums"])
+def test_rmsnorm_with_a_residual_equals_addition_and_norm(mode):
+    """RMSNorm.forward(residual=) and backward(stream_delta=) against triton_add_shortcut,
+    the plain layer and triton_delta_merge, in every parameter mode."""
+    import triton_tagi as tt
+    from triton_tagi.layers.resblock import triton_add_shortcut
+
+    class Buffers:
+        def buffer(self, layer, numel, dtype):
+            layer.buf = torch.empty(numel, dtype=dtype, device=DEV)
+            return layer.buf
+
+        def ready(self, layer):
+            layer.told = True
+
+    D = 96
+    ma, Sa, mr, Sr, w, Sw = norm_inputs(60, D, 8)
+    shape = (5, 12, D)
+    ma, Sa, mr, Sr = (t.view(shape) for t in (ma, Sa, mr, Sr))
+    g = gen(13)
+    dm, dS, xm, xS = randn(g, *shape), -rand(g, *shape), randn(g, *shape), -rand(g, *shape)
+    a, b = tt.RMSNorm(D, device=DEV), tt.RMSNorm(D, device=DEV)
+    for layer in (a, b):
+        layer.mw, layer.Sw = w.clone(), Sw.clone()
+        layer._set_param_mode(mode, 2.0, Buffers())
+    hm, hS = mr.clone(), Sr.clone()
+    triton_add_shortcut(ma, Sa, hm, hS)
+    ref = a.forward(hm, hS)
+    got = b.forward(ma, Sa, residual=(mr, Sr))
+    assert torch.equal(b.stream[0], hm) and torch.equal(b.stream[1], hS)
+    for x, y in zip(got, ref):
+        assert (x - y).abs().max() <= 128 * U * y.abs().max()
+    r_m, r_S = a.backward(dm, dS)
+    triton_add_shortcut(xm, xS, r_m, r_S)
+    d_m, d_S = b.backward(dm, dS, stream_delta=(xm, xS))
+    assert d_m.shape == shape
+    assert (d_m - r_m).abs().max() <= 128 * U * r_m.abs().max()
+    assert (d_S - r_S).abs().max() <= 256 * U * r_S.abs().max()
+    if mode == "sums":
+        assert b.told and (b.buf - a.buf).abs().max() <= 256 * U * a.buf.abs().max()
+    elif mode == "deltas":
+        for n in ("delta_mw", "delta_Sw"):
+            x, y = getattr(b, n), getattr(a, n)
+            assert (x - y).abs().max() <= 256 * U * y.abs().max()
+        b.update(2.0)
+        assert not torch.equal(b.mw, w)
+    else:
+        assert (b.mw - a.mw).abs().max() <= 256 * U * a.mw.abs().max()
+        assert (b.Sw - a.Sw).abs().max() <= 256 * U * a.Sw.abs().max()
+    plain = tt.RMSNorm(D, device=DEV)
+    plain.forward(ma, Sa)
+    with pytest.raises(ValueError, match="stream_delta"):
+        plain.backward(dm, dS, stream_delta=(xm, xS))
+
+
+def test_a_quantized_network_serves_its_predictions():
+    """Sequential.quantize(): predictions near the float32 network's, the fused 8-bit norm
+    equal to norm and quantization apart, and no training through it."""
+    import triton_tagi as tt
+    from triton_tagi.layers.int8_linear import Int8Linear
+
+    net = small_net(False, V=48, E=64)
+    x, y = small_batch(V=48)
+    for _ in range(3):
+        net.step(x, y, 0.05)
+    mu, var = net.forward(x)
+    served = net.quantize()
+    assert isinstance(served.layers[4], Int8Linear)
+    assert isinstance(served.layers[2].q_proj, Int8Linear)
+    assert isinstance(net.layers[4], tt.Linear) and isinstance(net.layers[2].q_proj, tt.Linear)
+    q_mu, q_var = served.forward(x)
+    # half a step of 127 on both operands of each of five products in a row, the errors
+    # of 64 terms adding up at random: a few hundredths of the outputs' own size
+    rms = lambda t: t.double().square().mean().sqrt().item()  # noqa: E731
+    assert rms(q_mu - mu) <= 0.05 * rms(mu)
+    assert rms(q_var - var) <= 0.1 * rms(var)
+    assert (q_var > 0).all()
+    h = served.layers[2].forward(*served.layers[1].forward(
+        *served.layers[0].forward(x, torch.zeros_like(x))))
+    fused = served.layers[4].forward_int8(served.layers[3].forward_int8(*h), h[0].shape[:-1])
+    apart = served.layers[4].forward(*served.layers[3].forward(*h))
+    assert rms(fused[0] - apart[0]) <= 1e-3 * rms(apart[0])
+    assert rms(fused[1] - apart[1]) <= 1e-3 * rms(apart[1])
+    with pytest.raises(RuntimeError, match="serves forward"):
+        served.step(x, y, 0.05)
+    with pytest.raises(RuntimeError, match="no backward"):
+        served.layers[4].backward(mu, var)
+    served.layers[3].forward_int8(*h)
+    with pytest.raises(RuntimeError, match="32 bits"):
+        served.layers[3].backward(*h)
+    # serving in the middle of a pass of the network itself disturbs nothing
+    ref = net.layers[3].forward(*h)
+    kept = net.layers[3].ma_in
+    served.forward(x)
+    assert net.layers[3].ma_in is kept and net.layers[2].q_proj.ma_in is not None
+    assert torch.equal(net.layers[3].forward(*h)[0], ref[0])
+    codes = served.layers[4].weight.q_m.clone()
+    net.step(x, y, 0.05)  # it trains on, the served weights stay
+    assert torch.equal(codes, served.layers[4].weight.q_m)
+
+
+def test_a_served_network_replays_from_a_graph():
+    net = small_net(False)
+    x, _ = small_batch()
+    served = net.quantize()
+    ref = served.forward(x)
+    static = x.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        served.forward(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = served.forward(static)
+    other = x.flip(0).contiguous()
+    for inputs in (x, other, x):
+        static.copy_(inputs)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = served.forward(inputs)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    assert torch.equal(out[0], ref[0])
+
+
+@pytest.mark.parametrize("kw", [dict(out_scale=4.0), dict(sorted_grad=True)])
+def test_the_embedding_step_captured(kw):
+    """Sequential(cuda_graph=True) with the sorted gradient: replays equal eager steps."""
+    x, y = small_batch()
+    sorted_grad = kw.pop("sorted_grad", False)
+    nets = [small_net(sorted_grad, **kw) for _ in range(2)]
+    nets[1].cuda_graph = True
+    for k in range(4):
+        xb = x.roll(k, 0).contiguous()
+        a = nets[0].step(xb, y, 0.05)
+        b = nets[1].step(xb, y, 0.05)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(nets[0].layers[0].mw, nets[1].layers[0].mw)
+    assert torch.equal(nets[0].layers[0].Sw, nets[1].layers[0].Sw)
+    nets[1].release_graph()

@@ -5,7 +5,9 @@ container may apply between neighbours (the results are the layers' own):
   ReLU's Jacobian inside its backward, and the ReLU's own backward is skipped;
 * a Conv2D whose outputs reach a BatchNorm2D (directly or through that ReLU)
   takes its bias sums (the per-channel sums of its output deltas) from the
-  BatchNorm's backward launch instead of a pass of its own.
+  BatchNorm's backward launch instead of a pass of its own;
+* an RMSNorm directly before an Int8Linear (a network that serves) writes that
+  layer's 8-bit operand itself.
 
 Forward fusions of the ReLU were measured and dropped: applied in the epilogue
 of the contraction before it, the exp/erf of the rectified moments at the end of
@@ -24,14 +26,24 @@ from torch import Tensor
 from .base import Layer
 from .layers.batchnorm2d import BatchNorm2D
 from .layers.conv2d import Conv2D
+from .layers.int8_linear import Int8Linear
 from .layers.relu import ReLU
+from .layers.rms_norm import RMSNorm
 
 
 def forward_chain(layers, ma: Tensor, Sa: Tensor) -> tuple[Tensor, Tensor]:
-    for layer in layers:
+    codes = None  # the next layer's input in 8 bits, from the RMSNorm before it
+    for i, layer in enumerate(layers):
         if not isinstance(layer, Layer):
             raise TypeError(f"Unknown layer type: {type(layer)}")
-        ma, Sa = layer.forward(ma, Sa)
+        if codes is not None:
+            ma, Sa = layer.forward_int8(codes, ma.shape[:-1])
+            codes = None
+        elif (isinstance(layer, RMSNorm) and i + 1 < len(layers)
+                and isinstance(layers[i + 1], Int8Linear)):
+            codes = layer.forward_int8(ma, Sa)
+        else:
+            ma, Sa = layer.forward(ma, Sa)
     return ma, Sa
 
 

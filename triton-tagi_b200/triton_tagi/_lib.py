@@ -211,17 +211,17 @@ def check_cuda_f32(*ts: torch.Tensor) -> None:
 def check_f32(*ts: torch.Tensor | None) -> int:
     """Checks that the tensors (None: absent) are float32 on one CUDA device and
     returns its index."""
-    dev = -1
+    dev = None
     for t in ts:
         if t is None:
             continue
+        d = t.get_device()
         if t.dtype is not torch.float32:
             raise ValueError(f"expected float32 tensor, got {t.dtype}")
-        d = t.get_device()
         if d != dev:
-            if d < 0:
+            if d < 0:  # the CPU's
                 raise ValueError("triton_tagi (B200) tensors must live on a CUDA device")
-            if dev >= 0:
+            if dev is not None:
                 raise ValueError(f"tensors live on different devices (cuda:{dev} and cuda:{d})")
             dev = d
     return dev

@@ -19,7 +19,7 @@ from .int8 import Int8Moments, _pointers, empty_codes
 
 def _rows(name: str, mw: Tensor, Sw: Tensor | None, *ts: Tensor | None) -> tuple[int, int, int]:
     """(device, rows, width) of the tensors given (None: absent), after checking them."""
-    dev = check_f32(mw, Sw, *ts)
+    dev = check_f32(*ts, mw, Sw)
     first = ts[0]
     width = mw.numel()
     if width < 1 or Sw is not None and Sw.numel() != width:

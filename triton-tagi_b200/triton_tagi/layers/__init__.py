@@ -5,6 +5,7 @@ from .batchnorm2d import BatchNorm2D
 from .conv2d import Conv2D
 from .embedding import Embedding
 from .flatten import Flatten
+from .int8_linear import Int8Linear
 from .linear import Linear
 from .multihead_attention import MultiheadAttentionV2
 from .positional_encoding import PositionalEncoding
@@ -13,5 +14,6 @@ from .remax import Remax
 from .resblock import Add, ResBlock
 from .rms_norm import RMSNorm
 
-__all__ = ["Add", "AvgPool2D", "BatchNorm2D", "Conv2D", "Embedding", "Flatten", "Linear",
+__all__ = ["Add", "AvgPool2D", "BatchNorm2D", "Conv2D", "Embedding", "Flatten", "Int8Linear",
+           "Linear",
            "MultiheadAttentionV2", "PositionalEncoding", "RMSNorm", "ReLU", "Remax", "ResBlock"]

@@ -73,6 +73,12 @@ class Linear(LearnableLayer):
         shp = (*self._input_shape[:-1], K)
         return d_ma.reshape(shp), d_Sa.reshape(shp)
 
+    def quantize(self):
+        """This layer as it is now for serving: an ``Int8Linear`` (inference only)."""
+        from .int8_linear import Int8Linear
+
+        return Int8Linear(self)
+
     def update(self, cap_factor: float) -> None:
         weight_update(self, cap_factor, self.has_bias)
 

@@ -12,6 +12,7 @@ the scale s, then the three projection backwards summed.
 
 from __future__ import annotations
 
+import copy
 import math
 
 import torch
@@ -19,6 +20,7 @@ from torch import Tensor
 
 from ..base import LearnableLayer
 from ..kernels.attention import bmm_shared_left, bmm_shared_right, bmm_tagi_moments
+from .int8_linear import Int8Linear
 from .linear import Linear
 from .relu import jacobian_backward
 from .remax import triton_remax
@@ -63,9 +65,15 @@ class MultiheadAttentionV2(LearnableLayer):
             raise ValueError(f"Expected last dim {self.embed_dim}, got {E}")
         H, D = self.num_heads, self.head_dim
         heads = lambda t: t.reshape(B, S, H, D).transpose(1, 2).contiguous()  # noqa: E731
-        mq, Sq = map(heads, self.q_proj.forward(ma, Sa))
-        mk, Sk = map(heads, self.k_proj.forward(ma, Sa))
-        mv, Sv = map(heads, self.v_proj.forward(ma, Sa))
+        if isinstance(self.q_proj, Int8Linear):  # serving: the input in 8 bits once
+            x = self.q_proj.codes(ma, Sa)
+            q, k, v = (p.forward_int8(x, ma.shape[:-1])
+                       for p in (self.q_proj, self.k_proj, self.v_proj))
+        else:
+            q, k, v = (p.forward(ma, Sa) for p in (self.q_proj, self.k_proj, self.v_proj))
+        mq, Sq = map(heads, q)
+        mk, Sk = map(heads, k)
+        mv, Sv = map(heads, v)
         s = self._scale
         mu_qk, var_qk = bmm_tagi_moments(mq, Sq, mk.transpose(-1, -2), Sk.transpose(-1, -2),
                                          s, s * s)
@@ -93,6 +101,15 @@ class MultiheadAttentionV2(LearnableLayer):
         b = self.k_proj.backward(back(dmk), back(dSk))
         v = self.v_proj.backward(back(dmv), back(dSv))
         return a[0] + b[0] + v[0], a[1] + b[1] + v[1]
+
+    def quantize(self) -> "MultiheadAttentionV2":
+        """This layer as it is now for serving: its projections in 8 bits (inference
+        only)."""
+        new = copy.copy(self)
+        new.q_proj, new.k_proj, new.v_proj = (p.quantize() for p in
+                                              (self.q_proj, self.k_proj, self.v_proj))
+        new._cache = new._attn_mu = new._attn_var = None
+        return new
 
     def update(self, cap_factor: float) -> None:
         for p in (self.q_proj, self.k_proj, self.v_proj):

@@ -5,6 +5,11 @@ Per row over the feature dim (rms_norm.py:93-110):
     μ_z = inv μ_a μ_γ,   S_z = inv² (S_a (μ_γ² + S_γ) + S_γ μ_a²)
 Backward (rms_norm.py:115-128): δμ_a = inv μ_γ δμ_z, δS_a = (inv μ_γ)² δS_z;
 γ sums Σ inv μ_a δμ_z and Σ inv² μ_a² δS_z over rows (float64).
+
+``forward(ma, Sa, residual=(mr, Sr))`` adds a residual stream first and keeps the sum in
+``stream``, in one pass (kernels/norm.py); ``backward(dmz, dSz, stream_delta=(dm, dS))``
+then adds the deltas that reached the stream behind the norm and returns the deltas of
+both addends. ``forward_int8`` gives the output in 8 bits for ``Int8Linear`` (no backward).
 """
 
 from __future__ import annotations
@@ -14,6 +19,9 @@ from torch import Tensor
 
 from .._lib import WGRAD_DELTAS, WGRAD_UPDATE, check_cuda_f32, lib, stream
 from ..base import LearnableLayer
+from ..kernels.int8 import Int8Moments
+from ..kernels.norm import (add_rmsnorm, add_rmsnorm_backward, add_rmsnorm_backward_sums,
+                            add_rmsnorm_backward_update, add_rmsnorm_int8)
 from ..param_init import init_weight_bias_norm
 from ._params import contiguous_params
 
@@ -37,13 +45,21 @@ class RMSNorm(LearnableLayer):
         self.mb = self.Sb = None
         self.ma_in = None
         self.inv_rms = None
+        self.stream = None  # (means, variances) of input plus residual, when one was given
         self._input_shape = None
         self.delta_mw = self.delta_Sw = self.delta_mb = self.delta_Sb = None
 
-    def forward(self, ma: Tensor, Sa: Tensor) -> tuple[Tensor, Tensor]:
+    def forward(self, ma: Tensor, Sa: Tensor,
+                residual: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
         check_cuda_f32(ma, Sa)
         contiguous_params(self, ("mw", "Sw"))
         self._input_shape = ma.shape
+        self.stream = None
+        if residual is not None:
+            hm, hS, mz, Sz, inv = add_rmsnorm(ma, Sa, *residual, self.mw, self.Sw, float(self.eps))
+            self.stream = (hm, hS)
+            self.ma_in, self.inv_rms = hm.view(-1, self.ni), inv.view(-1, 1)
+            return mz, Sz
         a = ma.reshape(-1, self.ni).contiguous()
         s = Sa.reshape(-1, self.ni).contiguous()
         rows = a.shape[0]
@@ -56,8 +72,44 @@ class RMSNorm(LearnableLayer):
         self.ma_in, self.inv_rms = a, inv
         return mz.reshape(self._input_shape), Sz.reshape(self._input_shape)
 
-    def backward(self, delta_mz: Tensor, delta_Sz: Tensor) -> tuple[Tensor, Tensor]:
+    def forward_int8(self, ma: Tensor, Sa: Tensor,
+                     residual: tuple[Tensor, Tensor] | None = None) -> Int8Moments:
+        """The output in 8 bits, leading dimensions flattened to rows (inference only:
+        nothing is kept for a backward but ``stream``)."""
+        contiguous_params(self, ("mw", "Sw"))
+        mr, Sr = (None, None) if residual is None else residual
+        hm, hS, q = add_rmsnorm_int8(ma, Sa, mr, Sr, self.mw, self.Sw, float(self.eps))
+        self.stream = None if residual is None else (hm, hS)
+        self.ma_in = self.inv_rms = None
+        return q
+
+    def _fused_backward(self, dmz, dSz, delta) -> tuple[Tensor, Tensor]:
+        mode = self._param_mode
+        head = (dmz, dSz, self.ma_in, self.inv_rms)
+        rm, rS = (None, None) if delta is None else delta
+        if mode == "deltas":
+            d_m, d_S, self.delta_mw, self.delta_Sw = add_rmsnorm_backward(
+                *head, self.mw, self.Sw, rm, rS)
+        elif mode == "update":
+            d_m, d_S = add_rmsnorm_backward_update(*head, self.mw, self.Sw, self._cap, rm, rS)
+            self._updated_in_backward = True
+        elif mode == "sums":
+            sums = self._reducer.buffer(self, 2 * self.ni, torch.float64)
+            d_m, d_S = add_rmsnorm_backward_sums(*head, self.mw, sums, rm, rS)
+            self._reducer.ready(self)
+        else:
+            raise ValueError(f"unknown parameter mode {mode!r}")
+        return d_m, d_S
+
+    def backward(self, delta_mz: Tensor, delta_Sz: Tensor,
+                 stream_delta: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
         check_cuda_f32(delta_mz, delta_Sz)
+        if self.ma_in is None:
+            raise RuntimeError("RMSNorm.backward needs a forward pass in 32 bits before it")
+        if self.stream is not None:
+            return self._fused_backward(delta_mz, delta_Sz, stream_delta)
+        if stream_delta is not None:
+            raise ValueError("RMSNorm.backward: stream_delta without a residual in the forward")
         shape = delta_mz.shape
         dm = delta_mz.reshape(-1, self.ni).contiguous()
         dS = delta_Sz.reshape(-1, self.ni).contiguous()

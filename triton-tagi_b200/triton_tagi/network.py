@@ -32,10 +32,14 @@ layer's training flag, so ``train()`` / ``eval()`` lead to a new capture.
 the tensor-core kernels' error word after every step (this synchronises) and
 raises ``RuntimeError`` if a bounded wait inside a kernel ran out, in which case
 that kernel's outputs are incomplete.
+
+``quantize()`` gives a network for serving: the same layers with every ``Linear`` (and
+the projections of attention layers) in 8 bits, for ``forward`` only.
 """
 
 from __future__ import annotations
 
+import copy
 import os
 
 import torch
@@ -44,6 +48,7 @@ from torch import Tensor
 from ._chain import backward_chain, forward_chain
 from ._lib import check_device_status
 from .base import LearnableLayer
+from .layers.linear import Linear
 from .layers.multihead_attention import MultiheadAttentionV2
 from .layers.resblock import ResBlock
 from .update.observation import compute_innovation
@@ -62,6 +67,7 @@ class Sequential:
         self.check_device = check_device
         self._graph = None  # (key, CUDAGraph or None, static x, static y, outputs)
         self.reducer = None  # set by triton_tagi.distributed.DataParallel
+        self.serving = False  # a network from quantize(): forward only
         for layer in self.layers:
             if isinstance(layer, ResBlock):
                 layer.device = self.device
@@ -100,7 +106,21 @@ class Sequential:
     def forward(self, x: Tensor) -> tuple[Tensor, Tensor]:
         return forward_chain(self.layers, x, torch.zeros_like(x))
 
+    def quantize(self) -> "Sequential":
+        """A network that serves this one's predictions from 8-bit weights: its ``Linear``
+        layers and attention projections as they are now, laid out once (``Int8Linear``).
+        The other layers are copies that share their parameters with this network, so
+        quantize again after training on. Only ``forward`` works on it."""
+        net = copy.copy(self)
+        net.layers = [layer.quantize() if isinstance(layer, (Linear, MultiheadAttentionV2))
+                      else copy.copy(layer) for layer in self.layers]
+        net.serving, net.reducer, net._graph = True, None, None
+        return net
+
     def step(self, x_batch: Tensor, y_batch: Tensor, sigma_v: float) -> tuple[Tensor, Tensor]:
+        if self.serving:
+            raise RuntimeError("a quantized network serves forward passes only; train the "
+                               "network that it was made from")
         red = self.reducer
         if self.cuda_graph and x_batch.is_cuda and (
                 red is None or getattr(red, "capturable", False)):
