@@ -177,6 +177,26 @@ def test_empty_batch_of_tokens():
     assert (mw == 1).all() and (Sw == 1).all()
 
 
+def test_update_of_deltas_that_are_not_numbers():
+    """As update_parameters: a NaN delta leaves its parameter, an infinite one moves it by
+    the cap."""
+    from triton_tagi.kernels import embedding_update
+    from triton_tagi.update.parameters import update_parameters
+
+    ids = torch.arange(4, device=DEV)
+    dm, dS = torch.zeros(4, 4, device=DEV), torch.zeros(4, 4, device=DEV)
+    dm[0, 0], dS[0, 1] = float("nan"), float("nan")
+    dm[1, 0], dS[1, 1] = float("inf"), -float("inf")
+    dm[2, 2] = -float("inf")
+    mw, Sw = torch.ones(6, 4, device=DEV), torch.full((6, 4), 0.25, device=DEV)
+    m2, S2 = mw[:4].clone(), Sw[:4].clone()
+    update_parameters(m2, S2, S2 * dm, S2 * S2 * dS, 2.0)
+    embedding_update(ids, dm, dS, mw, Sw, 2.0)
+    assert torch.isfinite(mw).all() and torch.isfinite(Sw).all()
+    assert torch.equal(mw[:4], m2) and torch.equal(Sw[:4], S2)
+    assert (mw[4:] == 1).all() and (Sw[4:] == 0.25).all()
+
+
 # -- residual RMSNorm ---------------------------------------------------------------
 
 ROWS = [(1, 1), (3, 5), (130, 64), (7, 127), (5, 128), (33, 512), (9, 1001), (4, 2048),
@@ -365,6 +385,18 @@ def test_add_rmsnorm_backward(R, D, stream):
     assert torch.equal(w1, w2) and torch.equal(S1, S2)
 
 
+def test_no_rows():
+    from triton_tagi.kernels import add_rmsnorm, add_rmsnorm_backward, add_rmsnorm_int8
+
+    e, w = torch.empty(0, 3, 64, device=DEV), torch.ones(64, device=DEV)
+    hm, hS, mz, Sz, inv = add_rmsnorm(e, e, e, e, w, w)
+    assert mz.shape == (0, 3, 64) and inv.shape == (0, 3)
+    q = add_rmsnorm_int8(e, e, e, e, w, w)[2]
+    assert q.q_m.shape == (0, 64) and q.values()[0].shape == (0, 64)
+    d_m, _, d_w, d_Sw = add_rmsnorm_backward(e, e, hm, inv, w, w, e, e)
+    assert d_m.shape == e.shape and not d_w.any() and not d_Sw.any()
+
+
 def test_backward_is_the_derivative_with_the_rms_held():
     """The deltas are J dmz and J^2 dSz with J = d mz / d h_m at a fixed 1/rms, as
     differences of the plain norm give it."""
@@ -442,6 +474,21 @@ def test_int8_moments_matmul_largest_sums():
     with pytest.raises(ValueError, match="33025"):
         big = operand(gen(1), 2, 33026)
         int8_moments_matmul(big, big)
+
+
+def test_a_token_gives_the_same_result_in_every_batch():
+    """1, 20, 40, 200 and 2100 tokens take different tiles and shares of the reduction; the
+    integer sums are exact and the rest is rounded alike."""
+    from triton_tagi.kernels import Int8Moments, int8_moments_matmul
+
+    g = gen(14)
+    x, w = operand(g, 2100, 1500), operand(g, 1300, 1500)
+    mb, Sb = randn(g, 1300), rand(g, 1300)
+    mz, Sz = int8_moments_matmul(x, w, mb, Sb)
+    for n in (1, 20, 40, 200):
+        part = Int8Moments(*(q[:n] for q in x[:3]), x.scales[:, :n])
+        a, b = int8_moments_matmul(part, w, mb, Sb)
+        assert torch.equal(a, mz[:n]) and torch.equal(b, Sz[:n])
 
 
 def test_int8_operands_of_other_layouts():
@@ -654,6 +701,39 @@ def test_a_scaled_embedding_equals_a_scaled_table():
     within(emb.delta_Sw, W * W * r_S, 36 * U * W * W * t_S, "delta_Sw")
 
 
+def test_a_sorted_gradient_for_a_reducer():
+    """Under data parallelism the raw sums go to the reducer's buffer, and the update is
+    applied from there."""
+    import triton_tagi as tt
+
+    class Buffers:
+        def buffer(self, layer, numel, dtype):
+            self.buf = torch.full((numel,), 7.0, dtype=dtype, device=DEV)
+            return self.buf
+
+        def ready(self, layer):
+            self.told = layer
+
+    emb = tt.Embedding(33, 7, device=DEV, sorted_grad=True)
+    g = gen(21)
+    ids = torch.randint(0, 33, (4, 9), device=DEV, generator=g).float()
+    emb.forward(ids, torch.zeros_like(ids))
+    red = Buffers()
+    emb._set_param_mode("sums", 2.0, red)
+    dm, dS = randn(g, 4, 9, 7), -rand(g, 4, 9, 7)
+    emb.backward(dm, dS)
+    assert red.told is emb
+    r_m, r_S, t_m, t_S = plain_sums(ids.view(-1), dm.view(-1, 7), dS.view(-1, 7), 33, -1, 1.0)
+    got = red.buf.view(2, 33, 7)
+    within(got[0], r_m, 34 * U * t_m, "sums of the means")
+    within(got[1], r_S, 34 * U * t_S, "sums of the variances")
+    m0 = emb.mw.clone()
+    emb.update(2.0)
+    assert torch.equal(emb.mw, m0)  # the reducer applies them
+    emb._apply_sums(red.buf, 2.0)
+    assert not torch.equal(emb.mw, m0)
+
+
 @pytest.mark.parametrize("mode", ["deltas", "update", "sums"])
 def test_rmsnorm_with_a_residual_equals_addition_and_norm(mode):
     """RMSNorm.forward(residual=) and backward(stream_delta=) against triton_add_shortcut,
@@ -721,6 +801,9 @@ def test_a_quantized_network_serves_its_predictions():
         net.step(x, y, 0.05)
     mu, var = net.forward(x)
     served = net.quantize()
+    twice = served.quantize()
+    assert all(a is b for a, b in zip((twice.layers[4], twice.layers[2].q_proj),
+                                      (twice.layers[4], served.layers[2].q_proj)))
     assert isinstance(served.layers[4], Int8Linear)
     assert isinstance(served.layers[2].q_proj, Int8Linear)
     assert isinstance(net.layers[4], tt.Linear) and isinstance(net.layers[2].q_proj, tt.Linear)

@@ -149,3 +149,5 @@ def test_layers_describe_themselves_and_refuse():
                      residual=(torch.zeros(2, 4), torch.zeros(2, 4)))
     with pytest.raises(ValueError, match="CUDA"):
         tt.Linear(4, 3, device="cpu").quantize()
+    with pytest.raises(ValueError, match="33025"):
+        tt.Linear(33026, 1, device="cpu").quantize()

@@ -609,9 +609,10 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
         const int m = m0 + c;
         if (n >= g.N || m >= g.M) return;
         const int64_t o = static_cast<int64_t>(m) * g.N + n;
-        g.Sz[o] = scale[0][c] * b[0] * static_cast<float>(a0) +
-                  scale[1][c] * b[1] * static_cast<float>(a1) + Sb;
-        g.mz[o] = scale[2][c] * b[2] * static_cast<float>(a2) + mb;
+        // rounded as the pair kernel does: a token's result does not depend on the batch
+        g.Sz[o] = fmaf(scale[1][c] * static_cast<float>(a1), b[1],
+                       fmaf(scale[0][c] * static_cast<float>(a0), b[0], Sb));
+        g.mz[o] = fmaf(scale[2][c] * static_cast<float>(a2), b[2], mb);
     };
     if (ctas == 1) {
         if (ok) {

@@ -20,7 +20,12 @@ from ..kernels.int8 import Int8Moments, int8_moments_matmul, quantize_moments, q
 class Int8Linear(Layer):
     """Made by ``Linear.quantize()``; ``Sequential.quantize()`` does so for a network."""
 
+    MAX_IN = 33025  # 255 * 255 * MAX_IN < 2^31: the integer sums hold every reduction
+
     def __init__(self, linear) -> None:
+        if linear.in_features > self.MAX_IN:
+            raise ValueError(f"Int8Linear: in_features={linear.in_features} exceeds {self.MAX_IN}, "
+                             "the longest reduction that 32-bit sums hold")
         self.in_features, self.out_features = linear.in_features, linear.out_features
         self.has_bias = linear.has_bias
         self.device = linear.mw.device

@@ -106,8 +106,9 @@ class MultiheadAttentionV2(LearnableLayer):
         """This layer as it is now for serving: its projections in 8 bits (inference
         only)."""
         new = copy.copy(self)
-        new.q_proj, new.k_proj, new.v_proj = (p.quantize() for p in
-                                              (self.q_proj, self.k_proj, self.v_proj))
+        new.q_proj, new.k_proj, new.v_proj = (
+            p.quantize() if isinstance(p, Linear) else p
+            for p in (self.q_proj, self.k_proj, self.v_proj))
         new._cache = new._attn_mu = new._attn_var = None
         return new
 
