@@ -149,9 +149,16 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::
                      : "memory");
 }
-__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+// A word of another CTA's shared memory, or 0 without reading; no branch, so that many
+// are in flight together.
+__device__ __forceinline__ int ld_cluster(uint32_t addr, bool read) {
     int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.s32 %0, 0;\n\t"
+        "@p ld.shared::cluster.s32 %0, [%1];\n\t}"
+        : "=r"(v)
+        : "r"(addr), "r"(read ? 1 : 0)
+        : "memory");
     return v;
 }
 // Tile copy from this GPU's own memory to this block alone. x is a multiple of kBK
@@ -513,15 +520,29 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
     const Abort ab{&abort_flag, 0};
     launch_dependents();
 
+    // item i of this CTA's list into its stage
+    auto issue = [&](int i) {
+        const int it = i - beg, s = it % P::STAGES;
+        const int p = i / kblocks, k = (i - p * kblocks) * kBK;
+        const uint32_t dst = smem_u32(smem + s * P::STAGE);
+        mbar_expect_tx(&full[s], P::STAGE);
+        tma_load(dst, &maps.w[w_of(p)], k, n0, &full[s]);
+        tma_load(dst + 128 * kBK, &maps.x[x_of(p)], k, m0, &full[s]);
+    };
+    int issued = beg;  // warp 0, lane 0
     if (threadIdx.x == 0) {
         for (int s = 0; s < P::STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         mbar_init(&done, 1);
-        abort_flag = g_int8_force_abort;
-        if (abort_flag) atomicCAS(&g_int8_error, 0, 2);
+        const int give_up = g_int8_force_abort;
+        abort_flag = give_up;
+        if (give_up) atomicCAS(&g_int8_error, 0, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // the first stages fill while the others set up
+        wait_for_primary();
+        for (; !give_up && issued < end && issued < beg + P::STAGES; ++issued) issue(issued);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -538,20 +559,16 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
 
     if (warp == 0) {
         if (lane == 0) {
-            int it = 0;
-            for (int i = beg; i < end; ++i, ++it) {
-                const int s = it % P::STAGES;
-                if (*ab.flag || (it >= P::STAGES &&
-                                 !mbar_wait(&empty[s], ((it / P::STAGES) - 1) & 1, ab, 11)))
+            for (; issued < end; ++issued) {
+                const int it = issued - beg;
+                if (*ab.flag || (it >= P::STAGES && !mbar_wait(&empty[it % P::STAGES],
+                                                               ((it / P::STAGES) - 1) & 1, ab, 11)))
                     break;
-                const int p = i / kblocks, k = (i - p * kblocks) * kBK;
-                const uint32_t dst = smem_u32(smem + s * P::STAGE);
-                mbar_expect_tx(&full[s], P::STAGE);
-                tma_load(dst, &maps.w[w_of(p)], k, n0, &full[s]);
-                tma_load(dst + 128 * kBK, &maps.x[x_of(p)], k, m0, &full[s]);
+                issue(issued);
             }
             // copies still in flight (after an abort) land before the CTA may exit
-            for (int i = it > P::STAGES ? it - P::STAGES : 0; i < it; ++i)
+            const int n = issued - beg;
+            for (int i = n > P::STAGES ? n - P::STAGES : 0; i < n; ++i)
                 if (!mbar_drain(&full[i % P::STAGES], (i / P::STAGES) & 1))
                     atomicCAS(&g_int8_error, 0, 13);
         }
@@ -650,24 +667,31 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
         __syncwarp();
         cluster_sync();
         if (reader && ok) {
-            // this CTA adds the columns [c0, c1), kWide at a time: the remote loads of
-            // all CTAs that hold a product are in flight together
-            constexpr int kWide = BN >= 64 ? 4 : 2;
+            // this CTA adds the columns [c0, c1), kWide at a time; the loads of two CTAs
+            // are in flight together
+            constexpr int kWide = BN >= 64 ? 8 : 2;
             const int c0 = share(BN, rank, ctas), c1 = share(BN, rank + 1, ctas);
             const uint32_t at0 = smem_u32(&sums[ch]);
             for (int c = c0; c < c1; c += kWide) {
                 int a[3][kWide] = {};
+#pragma unroll 1
+                for (int r0 = 0; r0 < ctas; r0 += 2) {  // ctas is 2, 4 or 8
+                    int v[2][3][kWide];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    if (r >= ctas) break;
-                    const uint32_t at = map_to(at0, r) + c * 512;
+                    for (int r = 0; r < 2; ++r) {
+                        const int bits = held[r0 + r];
+                        const uint32_t at = map_to(at0, r0 + r) + c * 512;
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        if (!(held[r] >> p & 1)) continue;
+                        for (int p = 0; p < 3; ++p)
 #pragma unroll
-                        for (int i = 0; i < kWide; ++i)
-                            if (c + i < c1) a[p][i] += ld_cluster(at + (p * BN + i) * 512);
+                            for (int i = 0; i < kWide; ++i)
+                                v[r][p][i] = ld_cluster(at + (p * BN + i) * 512,
+                                                        (bits >> p & 1) != 0 && c + i < c1);
                     }
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+#pragma unroll
+                        for (int i = 0; i < kWide; ++i) a[p][i] += v[0][p][i] + v[1][p][i];
                 }
 #pragma unroll
                 for (int i = 0; i < kWide; ++i)
