@@ -18,8 +18,8 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on, lib,
-                    ptr, workspace)
+from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on,
+                    empty_on, lib, ptr, workspace)
 
 _ID_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
@@ -31,9 +31,11 @@ def _id_type(ids: Tensor) -> int:
     return code
 
 
-def _check_table(mw: Tensor, Sw: Tensor) -> None:
-    if mw.dim() != 2 or mw.shape != Sw.shape:
-        raise ValueError(f"expected two (V, D) tables, got {tuple(mw.shape)} and {tuple(Sw.shape)}")
+def _check_table(mw: Tensor, Sw: Tensor) -> tuple[int, int]:
+    shape = mw.shape
+    if len(shape) != 2 or shape != Sw.shape:
+        raise ValueError(f"expected two (V, D) tables, got {tuple(shape)} and {tuple(Sw.shape)}")
+    return shape
 
 
 def embedding_lookup(ids: Tensor, mw: Tensor, Sw: Tensor, scale: float = 1.0,
@@ -42,13 +44,14 @@ def embedding_lookup(ids: Tensor, mw: Tensor, Sw: Tensor, scale: float = 1.0,
     code = _id_type(ids)
     dev = check_f32(mw, Sw)
     check_on(dev, ids)
-    _check_table(mw, Sw)
+    V, D = _check_table(mw, Sw)
     ids, mw, Sw = ids.contiguous(), mw.contiguous(), Sw.contiguous()
-    V, D = mw.shape
-    mz = mw.new_empty((*ids.shape, D))
-    Sz = torch.empty_like(mz)
+    n, shape = ids.numel(), ids.shape
+    mz, Sz = empty_on(dev, (n, D), (D, 1)), empty_on(dev, (n, D), (D, 1))
     call_on(dev, "tagi_embedding_lookup", ids.data_ptr(), code, mw.data_ptr(), Sw.data_ptr(),
-            mz.data_ptr(), Sz.data_ptr(), ids.numel(), V, D, padding_idx, scale)
+            mz.data_ptr(), Sz.data_ptr(), n, V, D, padding_idx, scale)
+    if len(shape) != 1:
+        mz, Sz = mz.view(*shape, D), Sz.view(*shape, D)
     return mz, Sz
 
 
@@ -97,9 +100,8 @@ def embedding_update(ids: Tensor, dmz: Tensor, dSz: Tensor, mw: Tensor, Sw: Tens
     """The capped update of (mw, Sw) from the deltas, in place, as ``update_parameters``
     with ``embedding_grad(..., Sw=Sw)`` would apply it to the rows that a token names;
     the other rows are neither read nor written."""
-    _check_table(mw, Sw)
+    V, D = _check_table(mw, Sw)
     if not (mw.is_contiguous() and Sw.is_contiguous()):
         raise ValueError("in-place targets must be contiguous")
-    V, D = mw.shape
     _grad(WGRAD_UPDATE, ids, dmz, dSz, V, D, float(scale), padding_idx, mw, Sw, None, None,
           float(cap_factor))

@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 from torch import Tensor
 
-from .._lib import call_on, check_f32, check_on, ptr
+from .._lib import call_on, check_f32, check_on, empty_on, ptr
 
 
 class Int8Moments(NamedTuple):
@@ -38,22 +38,22 @@ class Int8Moments(NamedTuple):
         """What the codes stand for: three float32 ``(rows, width)`` tensors."""
         dev = check_f32(self.scales)
         pointers, rows, width, _hold = _checked(self, dev)
-        new = self.scales.new_empty
-        v_m, v_2, v_S = new((rows, width)), new((rows, width)), new((rows, width))
+        size, stride = (rows, width), (width, 1)
+        v_m, v_2, v_S = (empty_on(dev, size, stride), empty_on(dev, size, stride),
+                         empty_on(dev, size, stride))
         call_on(dev, "tagi_int8_values", *pointers, v_m.data_ptr(), v_2.data_ptr(), v_S.data_ptr(),
                 rows, width)
         return v_m, v_2, v_S
 
 
-def empty_codes(rows: int, width: int, like: Tensor) -> Int8Moments:
+def empty_codes(rows: int, width: int, dev: int) -> Int8Moments:
     """Uninitialised codes whose rows start on 16-byte boundaries, as the tensor-core
     product's copies need them."""
-    ld = (width + 15) // 16 * 16
-    new = like.new_empty_strided
-    size, stride = (rows, width), (ld, 1)
-    return Int8Moments(new(size, stride, dtype=torch.int8), new(size, stride, dtype=torch.uint8),
-                       new(size, stride, dtype=torch.uint8),
-                       like.new_empty((3, rows), dtype=torch.float32))
+    size, stride = (rows, width), ((width + 15) // 16 * 16, 1)
+    return Int8Moments(empty_on(dev, size, stride, torch.int8),
+                       empty_on(dev, size, stride, torch.uint8),
+                       empty_on(dev, size, stride, torch.uint8),
+                       empty_on(dev, (3, rows), (rows, 1)))
 
 
 def _checked(q: Int8Moments, dev: int) -> tuple:
@@ -80,7 +80,7 @@ def _checked(q: Int8Moments, dev: int) -> tuple:
         same = stride[1] == 1 and q_2.stride() == stride and q_S.stride() == stride
     if not same or ld < width \
             or (ld | q_m.data_ptr() | q_2.data_ptr() | q_S.data_ptr()) & 15:
-        new = empty_codes(rows, width, scales)
+        new = empty_codes(rows, width, dev)
         new.q_m.copy_(q_m)
         new.q_2.copy_(q_2)
         new.q_S.copy_(q_S)
@@ -104,7 +104,7 @@ def _quantize(m: Tensor, S: Tensor, weights: bool) -> Int8Moments:
                          "shape and a last dimension")
     width = m.shape[-1]
     m, S = m.reshape(-1, width).contiguous(), S.reshape(-1, width).contiguous()
-    q = empty_codes(m.shape[0], width, m)
+    q = empty_codes(m.shape[0], width, dev)
     call_on(dev, "tagi_quantize_moments", m.data_ptr(), S.data_ptr(), 1 if weights else 0,
             *_pointers(q, width), m.shape[0], width)
     return q
@@ -136,8 +136,7 @@ def int8_moments_matmul(x: Int8Moments, w: Int8Moments, mb: Tensor | None = None
         raise ValueError(f"biases must hold {N} values")
     mb = None if mb is None else mb.contiguous()
     Sb = None if Sb is None else Sb.contiguous()
-    mz = x.scales.new_empty((M, N))
-    Sz = torch.empty_like(mz)
+    mz, Sz = empty_on(dev, (M, N), (N, 1)), empty_on(dev, (M, N), (N, 1))
     call_on(dev, "tagi_int8_moment_matmul", *px, *pw, ptr(mb), ptr(Sb),
             mz.data_ptr(), Sz.data_ptr(), M, N, K)
     return mz, Sz

@@ -12,8 +12,8 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on, lib,
-                    ptr, workspace)
+from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on,
+                    empty_on, lib, ptr, workspace)
 from .int8 import Int8Moments, _pointers, empty_codes
 
 
@@ -51,9 +51,12 @@ def add_rmsnorm(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | None, mw
     _pair("add_rmsnorm", mr, Sr)
     dev, rows, width = _rows("add_rmsnorm", mw, Sw, ma, Sa, mr, Sr)
     ma, Sa, mr, Sr, mw, Sw = _cont(ma, Sa, mr, Sr, mw, Sw)
-    hm, hS = (ma, Sa) if mr is None else (torch.empty_like(ma), torch.empty_like(Sa))
-    mz, Sz = torch.empty_like(ma), torch.empty_like(Sa)
-    inv = ma.new_empty(ma.shape[:-1])
+    size, stride = tuple(ma.shape), ma.stride()
+    hm, hS = (ma, Sa) if mr is None else (empty_on(dev, size, stride), empty_on(dev, size, stride))
+    mz, Sz = empty_on(dev, size, stride), empty_on(dev, size, stride)
+    inv = empty_on(dev, (rows,), (1,))
+    if len(size) != 2:
+        inv = inv.view(size[:-1])
     call_on(dev, "tagi_add_rmsnorm_forward", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
             mw.data_ptr(), Sw.data_ptr(), hm.data_ptr(), hS.data_ptr(), mz.data_ptr(),
             Sz.data_ptr(), inv.data_ptr(), rows, width, eps)
@@ -67,8 +70,9 @@ def add_rmsnorm_int8(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | Non
     _pair("add_rmsnorm_int8", mr, Sr)
     dev, rows, width = _rows("add_rmsnorm_int8", mw, Sw, ma, Sa, mr, Sr)
     ma, Sa, mr, Sr, mw, Sw = _cont(ma, Sa, mr, Sr, mw, Sw)
-    hm, hS = (ma, Sa) if mr is None else (torch.empty_like(ma), torch.empty_like(Sa))
-    q = empty_codes(rows, width, ma)
+    size, stride = tuple(ma.shape), ma.stride()
+    hm, hS = (ma, Sa) if mr is None else (empty_on(dev, size, stride), empty_on(dev, size, stride))
+    q = empty_codes(rows, width, dev)
     call_on(dev, "tagi_add_rmsnorm_int8", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
             mw.data_ptr(), Sw.data_ptr(), hm.data_ptr(), hS.data_ptr(), *_pointers(q, width), rows,
             width, eps)
@@ -84,7 +88,8 @@ def _backward(mode, dmz, dSz, hm, inv, mw, Sw, rm, rS, sums=None, d_mw=None, d_S
         raise ValueError(f"{name}: the stream {tuple(hm.shape)} and 1/rms {tuple(inv.shape)} do "
                          f"not match {rows} rows of {width}")
     dmz, dSz, hm, inv, rm, rS = _cont(dmz, dSz, hm, inv, rm, rS)
-    d_m, d_S = torch.empty_like(dmz), torch.empty_like(dSz)
+    size, stride = tuple(dmz.shape), dmz.stride()
+    d_m, d_S = empty_on(dev, size, stride), empty_on(dev, size, stride)
     hold, wp, wn = workspace(lib().size("tagi_add_rmsnorm_backward_workspace_size", rows, width),
                              dmz)
     call_on(dev, "tagi_add_rmsnorm_backward", dmz.data_ptr(), dSz.data_ptr(), hm.data_ptr(),
