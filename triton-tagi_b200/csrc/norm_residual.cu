@@ -190,7 +190,13 @@ __device__ __forceinline__ void codes(const Elem<OUT>& e, const RowScales& r, in
 }
 
 // One row per group of WARPS warps, its stream held in registers: thread i of the
-// group has vectors i, i + 32 WARPS, ... (NV at most).
+// group has vectors i, i + 32 WARPS, ... (NV at most). One pass over the inputs.
+//
+// Bound by HBM: 32 bytes per element (27 with codes). 8192 x 4096: 163 us, 6.6 TB/s, the
+// rate of a copy; 16384 x 512 with codes: 42 us, 5.4 TB/s. Forming the quotients of the
+// codes in fp32 and only those near the middle of two in double took as long (44 us):
+// the double arithmetic hides behind the loads. 777 x 1001, one element per load: 11 us,
+// bound by latency.
 template <int OUT, int VEC, int WARPS, int NV>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) row_kernel(const NormArgs g) {
     __shared__ RowStats red[WARPS];
@@ -420,7 +426,7 @@ int launch_norm(const NormArgs& g, cudaStream_t st, const char* what) {
 }
 
 // code * scale of one of the three operands (blockIdx.y), VEC codes per thread; the
-// block's y rows at a time.
+// block's y rows at a time. Bound by HBM: 16384 x 512 in 25 us, 6.0 TB/s.
 template <int VEC>
 __global__ void values_kernel(const NormArgs g, float* vm, float* v2, float* vS) {
     launch_dependents();
@@ -455,7 +461,9 @@ __global__ void values_kernel(const NormArgs g, float* vm, float* v2, float* vS)
 // Both are formed in one pass: block (slice, columns) walks its rows with its columns'
 // sums in registers, kBackThreads / x rows at a time (x threads along the columns), adds
 // the groups' sums in order and leaves them in the workspace; a second launch adds the
-// slices in order and applies them.
+// slices in order and applies them. Bound by HBM: 28 bytes per element. 16384 x 512:
+// 43.6 us with the second launch, 5.4 TB/s; without the row groups there were four times
+// the slices and the second launch alone took 15 us.
 constexpr int kBackThreads = 512;
 constexpr int kBackCols = 128;  // threads along the columns, at most
 
