@@ -63,7 +63,9 @@ struct Vec<1> { using type = float; };
 
 template <int VEC>
 __device__ __forceinline__ void ldv(const float* p, float (&v)[VEC]) {
-    const typename Vec<VEC>::type x = __ldg(reinterpret_cast<const typename Vec<VEC>::type*>(p));
+    // a plain load: the read-only path may not see what the kernel before this one, still
+    // running when this one is launched, writes
+    const typename Vec<VEC>::type x = *reinterpret_cast<const typename Vec<VEC>::type*>(p);
     const float* f = reinterpret_cast<const float*>(&x);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = f[e];
@@ -298,10 +300,8 @@ __device__ __forceinline__ void capped_step(float& m, float& S, float dm, float 
 template <int VEC, int MODE>
 __device__ __forceinline__ void params(const GradArgs& a, int64_t o, float (&mean)[VEC],
                                        float (&w)[VEC]) {
-    using T = typename Vec<VEC>::type;
-    if (MODE != TAGI_WGRAD_SUMS) *reinterpret_cast<T*>(w) = *reinterpret_cast<const T*>(a.Sw + o);
-    if (MODE == TAGI_WGRAD_UPDATE)
-        *reinterpret_cast<T*>(mean) = *reinterpret_cast<const T*>(a.mw + o);
+    if (MODE != TAGI_WGRAD_SUMS) ldv<VEC>(a.Sw + o, w);
+    if (MODE == TAGI_WGRAD_UPDATE) ldv<VEC>(a.mw + o, mean);
 }
 
 // The sums of one row at offset o in their final form.
