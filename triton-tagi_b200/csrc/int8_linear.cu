@@ -121,6 +121,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const 
                                           int code) {
     return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, ab, code);
 }
+// The same for a whole warp, so that what follows stays uniform.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab,
+                                          int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, code));
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 // For copies and MMAs in flight, which must land before the block may exit.
 __device__ __noinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
     const unsigned long long t0 = globaltimer();
@@ -257,6 +269,21 @@ __device__ __forceinline__ uint32_t instr_desc(bool sign, int m, int bn) {
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// Position in a ring of stages, and the parity of the use of the stage before this one.
+template <int STAGES>
+struct Ring {
+    int s = 0;
+    uint32_t parity = 0;  // of this use; the use before has the other
+    bool again = false;   // the stage has been used before
+    __device__ __forceinline__ void next() {
+        if (++s == STAGES) {
+            s = 0;
+            parity ^= 1u;
+            again = true;
+        }
+    }
+};
+
 // Products in their order: variance x_2 w_S, variance x_S w_2, mean x_m w_m; the index
 // of the operands and scales (0 means, 1 second operand, 2 variances).
 __device__ __forceinline__ int x_of(int product) { return product == 0 ? 1 : (product == 1 ? 2 : 0); }
@@ -317,78 +344,92 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     wait_for_primary();
     const uint32_t tmem = tmem_base;
 
+    // The copying and the multiplying warp run their loops whole and one elected lane
+    // issues: with operands in uniform registers an MMA costs its issuer a few clocks,
+    // from a loop of one lane it cost 100 (and the kernel half of its speed).
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;
-            bool alive = true;
-            for (int tile = blockIdx.x / 2; tile < tiles && alive; tile += pairs) {
-                const int n = (tile % ctiles) * 256 + static_cast<int>(rank) * 128;
-                const int m = (tile / ctiles) * 256 + static_cast<int>(rank) * 128;
-                for (int p = 0; p < 3 && alive; ++p) {
-                    const CUtensorMap* x = &maps.x[x_of(p)];
-                    const CUtensorMap* w = &maps.w[w_of(p)];
-                    for (int k = 0; k < kblocks; ++k, ++it) {
-                        const int s = it % kPairStages;
-                        if (*ab.flag || (it >= kPairStages &&
-                                         !mbar_wait(&empty[s], ((it / kPairStages) - 1) & 1, ab, 21))) {
-                            alive = false;
-                            break;
-                        }
-                        const uint32_t dst = smem_u32(smem + s * kPairStage);
-                        mbar_expect_tx(&landed[s], kPairStage);
-                        tma_load(dst, w, k * kBK, n, &landed[s]);
-                        tma_load(dst + 128 * kBK, x, k * kBK, m, &landed[s]);
+        const bool lead = elect_one();
+        Ring<kPairStages> ring;
+        int it = 0;
+        bool alive = true;
+        for (int tile = blockIdx.x / 2; tile < tiles && alive; tile += pairs) {
+            const int n = (tile % ctiles) * 256 + static_cast<int>(rank) * 128;
+            const int m = (tile / ctiles) * 256 + static_cast<int>(rank) * 128;
+#pragma unroll 1
+            for (int p = 0; p < 3 && alive; ++p) {
+                const CUtensorMap* x = &maps.x[x_of(p)];
+                const CUtensorMap* w = &maps.w[w_of(p)];
+#pragma unroll 1
+                for (int k = 0; k < kblocks; ++k, ++it, ring.next()) {
+                    alive = ring.again ? warp_wait(&empty[ring.s], ring.parity ^ 1u, ab, 21)
+                                       : __all_sync(0xffffffffu, *ab.flag == 0);
+                    if (!alive) break;
+                    if (lead) {
+                        uint64_t* bar = &landed[ring.s];
+                        const uint32_t dst = smem_u32(smem + ring.s * kPairStage);
+                        mbar_expect_tx(bar, kPairStage);
+                        tma_load(dst, w, k * kBK, n, bar);
+                        tma_load(dst + 128 * kBK, x, k * kBK, m, bar);
                     }
+                    __syncwarp();
                 }
             }
-            // copies still in flight (after an abort) land before the CTA may exit
-            for (int i = it > kPairStages ? it - kPairStages : 0; i < it; ++i)
-                if (!mbar_drain(&landed[i % kPairStages], (i / kPairStages) & 1))
-                    atomicCAS(&g_int8_error, 0, 23);
         }
+        // copies still in flight (after an abort) land before the CTA may exit
+        for (int i = it > kPairStages ? it - kPairStages : 0; i < it; ++i)
+            if (!mbar_drain(&landed[i % kPairStages], (i / kPairStages) & 1) && lane == 0)
+                atomicCAS(&g_int8_error, 0, 23);
     } else if (warp == 1) {
-        if (lane == 0 && rank != 0) {
+        if (rank != 0) {
             // tells the leader which stages have landed here
             const int my_tiles = (tiles - static_cast<int>(blockIdx.x / 2) + pairs - 1) / pairs;
             const int iters = my_tiles * 3 * kblocks;
-            for (int it = 0; it < iters; ++it) {
-                const int s = it % kPairStages;
-                if (!mbar_wait(&landed[s], (it / kPairStages) & 1, ab, 22)) break;
-                arrive_cluster(map_to(smem_u32(&peer_landed[s]), 0));
+            const uint32_t to = map_to(smem_u32(&peer_landed[0]), 0);
+            Ring<kPairStages> ring;
+#pragma unroll 1
+            for (int it = 0; it < iters; ++it, ring.next()) {
+                if (!warp_wait(&landed[ring.s], ring.parity, ab, 22)) break;
+                if (lane == 0) arrive_cluster(to + ring.s * 8);
             }
-        } else if (lane == 0) {
-            int it = 0, unit = 0;
+        } else {
+            const bool lead = elect_one();
+            Ring<kPairStages> ring;
+            int unit = 0;
             bool alive = true;
             for (int tile = blockIdx.x / 2; tile < tiles && alive; tile += pairs) {
+#pragma unroll 1
                 for (int p = 0; p < 3 && alive; ++p, ++unit) {
                     const uint32_t idesc = instr_desc(p == 2, 256, 256);
                     const int slot = unit & 1;
-                    if (unit >= 2 && !mbar_wait(&acc_empty[slot], ((unit / 2) - 1) & 1, ab, 24)) {
+                    if (unit >= 2 && !warp_wait(&acc_empty[slot], ((unit / 2) - 1) & 1, ab, 24)) {
                         alive = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t d = tmem + slot * 256;
-                    for (int k = 0; k < kblocks; ++k, ++it) {
-                        const int s = it % kPairStages;
-                        const uint32_t par = (it / kPairStages) & 1;
-                        if (!mbar_wait(&landed[s], par, ab, 25) ||
-                            !mbar_wait(&peer_landed[s], par, ab, 26)) {
-                            alive = false;
-                            break;
-                        }
+#pragma unroll 1
+                    for (int k = 0; k < kblocks; ++k, ring.next()) {
+                        alive = warp_wait(&landed[ring.s], ring.parity, ab, 25) &&
+                                warp_wait(&peer_landed[ring.s], ring.parity, ab, 26);
+                        if (!alive) break;
                         tc_fence_after();
-                        const uint32_t base = smem_u32(smem + s * kPairStage);
+                        const uint32_t base = smem_u32(smem + ring.s * kPairStage);
                         const uint64_t a = tile_desc(base), b = tile_desc(base + 128 * kBK);
+                        if (lead) {
+                            mma_i8<true>(d, a, b, idesc, k == 0 ? 0u : 1u);
 #pragma unroll
-                        for (int j = 0; j < kBK / 32; ++j)
-                            mma_i8<true>(d, a + 2 * j, b + 2 * j, idesc, k == 0 && j == 0 ? 0u : 1u);
-                        mma_commit_pair(&empty[s]);
+                            for (int j = 1; j < kBK / 32; ++j)
+                                mma_i8<true>(d, a + 2 * j, b + 2 * j, idesc, 1u);
+                            mma_commit_pair(&empty[ring.s]);
+                        }
+                        __syncwarp();
                     }
-                    if (alive) mma_commit_pair(&acc_full[slot]);
+                    if (alive && lead) mma_commit_pair(&acc_full[slot]);
+                    __syncwarp();
                 }
             }
-            mma_commit_pair(&done);
+            if (lead) mma_commit_pair(&done);
+            __syncwarp();
         }
     } else {
         const int quarter = warp & 3, part = (warp - 2) >> 2;  // columns part * 64 .. + 63
@@ -527,9 +568,8 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
     const Abort ab{&abort_flag, 0};
     launch_dependents();
 
-    // item i of this CTA's list into its stage
-    auto issue = [&](int i) {
-        const int it = i - beg, s = it % P::STAGES;
+    // item i of this CTA's list into stage s
+    auto issue = [&](int i, int s) {
         const int p = i / kblocks, k = (i - p * kblocks) * kBK;
         const uint32_t dst = smem_u32(smem + s * P::STAGE);
         mbar_expect_tx(&full[s], P::STAGE);
@@ -549,7 +589,7 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         // the first stages fill while the others set up
         wait_for_primary();
-        for (; !give_up && issued < end && issued < beg + P::STAGES; ++issued) issue(issued);
+        for (; !give_up && issued < end && issued < beg + P::STAGES; ++issued) issue(issued, issued - beg);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -565,38 +605,50 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
     wait_for_primary();
 
     if (warp == 0) {
-        if (lane == 0) {
-            for (; issued < end; ++issued) {
-                const int it = issued - beg;
-                if (*ab.flag || (it >= P::STAGES && !mbar_wait(&empty[it % P::STAGES],
-                                                               ((it / P::STAGES) - 1) & 1, ab, 11)))
-                    break;
-                issue(issued);
-            }
-            // copies still in flight (after an abort) land before the CTA may exit
-            const int n = issued - beg;
-            for (int i = n > P::STAGES ? n - P::STAGES : 0; i < n; ++i)
-                if (!mbar_drain(&full[i % P::STAGES], (i / P::STAGES) & 1))
-                    atomicCAS(&g_int8_error, 0, 13);
+        // lane 0, which set the barriers up, has filled the first stages already
+        int it = __shfl_sync(0xffffffffu, issued, 0) - beg;
+        Ring<P::STAGES> ring;
+        for (int i = 0; i < it; ++i) ring.next();
+#pragma unroll 1
+        for (; beg + it < end; ++it, ring.next()) {
+            if (!(ring.again ? warp_wait(&empty[ring.s], ring.parity ^ 1u, ab, 11)
+                             : __all_sync(0xffffffffu, *ab.flag == 0)))
+                break;
+            if (lane == 0) issue(beg + it, ring.s);
+            __syncwarp();
         }
+        // copies still in flight (after an abort) land before the CTA may exit
+        for (int i = it > P::STAGES ? it - P::STAGES : 0; i < it; ++i)
+            if (!mbar_drain(&full[i % P::STAGES], (i / P::STAGES) & 1) && lane == 0)
+                atomicCAS(&g_int8_error, 0, 13);
     } else if (warp == 1) {
-        if (lane == 0) {
-            for (int i = beg, it = 0; i < end; ++i, ++it) {
-                const int s = it % P::STAGES;
-                if (!mbar_wait(&full[s], (it / P::STAGES) & 1, ab, 12)) break;
-                tc_fence_after();
-                const int p = i / kblocks;
-                const uint32_t idesc = instr_desc(p == 2, 128, BN);
-                const uint32_t base = smem_u32(smem + s * P::STAGE);
-                const uint64_t a = tile_desc(base), b = tile_desc(base + 128 * kBK);
-                const bool first = i == beg || i == p * kblocks;
+        const bool lead = elect_one();
+        Ring<P::STAGES> ring;
+        int p = beg / kblocks, k = beg - p * kblocks;
+        bool first = true;  // of this CTA's blocks of the product
+#pragma unroll 1
+        for (int i = beg; i < end; ++i, ring.next()) {
+            if (!warp_wait(&full[ring.s], ring.parity, ab, 12)) break;
+            tc_fence_after();
+            const uint32_t idesc = instr_desc(p == 2, 128, BN);
+            const uint32_t base = smem_u32(smem + ring.s * P::STAGE);
+            const uint64_t a = tile_desc(base), b = tile_desc(base + 128 * kBK);
+            const uint32_t d = tmem + p * BN;
+            if (lead) {
+                mma_i8<false>(d, a, b, idesc, first ? 0u : 1u);
 #pragma unroll
-                for (int j = 0; j < kBK / 32; ++j)
-                    mma_i8<false>(tmem + p * BN, a + 2 * j, b + 2 * j, idesc, first && j == 0 ? 0u : 1u);
-                mma_commit(&empty[s]);
+                for (int j = 1; j < kBK / 32; ++j) mma_i8<false>(d, a + 2 * j, b + 2 * j, idesc, 1u);
+                mma_commit(&empty[ring.s]);
             }
-            mma_commit(&done);
+            __syncwarp();
+            first = ++k == kblocks;
+            if (first) {
+                k = 0;
+                ++p;
+            }
         }
+        if (lead) mma_commit(&done);
+        __syncwarp();
     } else {
         const int t = threadIdx.x - 64;
         if (t < ctas) {
