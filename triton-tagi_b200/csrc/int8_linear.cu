@@ -35,8 +35,8 @@
 //
 // Warp roles: warp 0 issues the tensor-map copies (128 bytes of the reduction of both
 // operands per stage, 128-byte swizzle), warp 1 allocates tensor memory and issues the
-// MMAs (in the second CTA of a pair it tells the first which stages have landed), the
-// others read the accumulators (lane quarter w % 4) and store.
+// MMAs (in a pair's first CTA, which a warp of both tells of the stages that have landed),
+// the others read the accumulators (lane quarter w % 4) and store.
 //
 // Every wait is bounded: on timeout a CTA records an error word (tagi_device_status),
 // tells its peer, stops issuing, lets its own copies and MMAs land and frees its tensor
@@ -294,12 +294,13 @@ constexpr int kPairStages = 6;
 constexpr int kPairStage = 2 * 128 * kBK;  // 128 channels and 128 tokens per CTA
 constexpr int kPairSmem = kPairStages * kPairStage + 1024;
 constexpr int kPairReaders = 16;  // epilogue warps: 4 per lane quarter, 64 columns each
-constexpr int kPairThreads = 64 + 32 * kPairReaders;
+constexpr int kTeller = 2 + kPairReaders;  // the warp that tells the leader of landed stages
+constexpr int kPairThreads = 32 * (kTeller + 1);
 
 __global__ void __launch_bounds__(kPairThreads, 1)
     int8_pair_kernel(const Int8Args g, const __grid_constant__ Maps maps) {
     extern __shared__ char raw[];
-    __shared__ __align__(8) uint64_t landed[kPairStages], peer_landed[kPairStages],
+    __shared__ __align__(8) uint64_t landed[kPairStages], ready[kPairStages],
         empty[kPairStages], acc_full[2], acc_empty[2], done;
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag;
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) {
             mbar_init(&landed[s], 1);
-            mbar_init(&peer_landed[s], 1);
+            mbar_init(&ready[s], 2);  // leader: the stage has landed in both CTAs
             mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -379,19 +380,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         for (int i = it > kPairStages ? it - kPairStages : 0; i < it; ++i)
             if (!mbar_drain(&landed[i % kPairStages], (i / kPairStages) & 1) && lane == 0)
                 atomicCAS(&g_int8_error, 0, 23);
-    } else if (warp == 1) {
-        if (rank != 0) {
-            // tells the leader which stages have landed here
-            const int my_tiles = (tiles - static_cast<int>(blockIdx.x / 2) + pairs - 1) / pairs;
-            const int iters = my_tiles * 3 * kblocks;
-            const uint32_t to = map_to(smem_u32(&peer_landed[0]), 0);
-            Ring<kPairStages> ring;
+    } else if (warp == kTeller) {
+        // one barrier for the multiplying warp to wait on instead of one per CTA
+        const int my_tiles = (tiles - static_cast<int>(blockIdx.x / 2) + pairs - 1) / pairs;
+        const int iters = my_tiles * 3 * kblocks;
+        const uint32_t to = map_to(smem_u32(&ready[0]), 0);
+        Ring<kPairStages> ring;
 #pragma unroll 1
-            for (int it = 0; it < iters; ++it, ring.next()) {
-                if (!warp_wait(&landed[ring.s], ring.parity, ab, 22)) break;
-                if (lane == 0) arrive_cluster(to + ring.s * 8);
-            }
-        } else {
+        for (int it = 0; it < iters; ++it, ring.next()) {
+            if (!warp_wait(&landed[ring.s], ring.parity, ab, 22)) break;
+            if (lane == 0) arrive_cluster(to + ring.s * 8);
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
             const bool lead = elect_one();
             Ring<kPairStages> ring;
             int unit = 0;
@@ -409,8 +410,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     const uint32_t d = tmem + slot * 256;
 #pragma unroll 1
                     for (int k = 0; k < kblocks; ++k, ring.next()) {
-                        alive = warp_wait(&landed[ring.s], ring.parity, ab, 25) &&
-                                warp_wait(&peer_landed[ring.s], ring.parity, ab, 26);
+                        alive = warp_wait(&ready[ring.s], ring.parity, ab, 25);
                         if (!alive) break;
                         tc_fence_after();
                         const uint32_t base = smem_u32(smem + ring.s * kPairStage);
