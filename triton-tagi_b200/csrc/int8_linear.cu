@@ -15,23 +15,22 @@
 //
 // pair kernel, for many tokens. A cluster of two CTAs computes 256 channels x 256
 // tokens with 2-SM MMAs: each CTA stages its 128 channels and half of the tokens, 64
-// bytes per clock of the tensor pipe's peak and SM (a single-CTA 128 x 128 tile stages
-// 128 and took 433 us for 8192 x 4096 x 4096). Persistent, one pair per two SMs. The
+// bytes per clock of the tensor pipe's peak and SM, which the L2 delivers (a single-CTA
+// 128 x 128 tile stages 128). Persistent, one pair per two SMs. The
 // three products of a tile follow one another through two accumulators of 256 columns:
 // the epilogue warps read one while the MMAs fill the other. The first product of the
 // variance waits in their registers for the second.
-//   8192 x 4096 x 4096: 297 us, 2.8 POP/s (355 us, under the power cap, in a loop). Bound
-//   by the L2: the tiles are 3.2 GB of it, 11 TB/s; the tensor pipe is 70 % active.
-//   16384 x 512 x 2048: 72 us (82 in a loop), bound by the L2 as well: 402 MB of tiles
-//   and 268 MB of outputs, whose stores fill the time of the MMAs.
+//   8192 x 4096 x 4096: 257 us, 3.2 POP/s; the tensor pipe is active 84 % of the cycles
+//   at the 1.6 GHz that its power leaves (348 us in a loop, under the power cap).
+//   16384 x 512 x 2048: 67.5 us (80 in a loop), bound by the epilogue, 12 thousand clocks
+//   a tile against 6 of MMAs: 37 us without it, 57 with all of it but the stores.
 //
-// split kernel, for few tokens or few tiles. 128 channels x BN tokens (BN from 16);
+// split kernel, for few tokens or few tiles. 128 channels x BN tokens (16 or 32);
 // the (product, reduction block) list of a tile is shared out over a cluster of up to
 // 8 CTAs, which exchange their integer sums through distributed shared memory (exact in
 // any order).
-//   16 x 4096 x 4096: 20 us, the 50 MB of weights at 5.2 TB/s while they stream, the
-//   rest set-up and exchange. 3 x 2048 x 512: 10 us, latency: set-up 1 us, first tile 1.3,
-//   five more 2, exchange and stores 2.5.
+//   16 x 4096 x 4096: 17 us for 50 MB of weights. 3 x 2048 x 512: 9 us of latency: set-up
+//   and first tile 2 us, the others 2, exchange and stores 2.
 //
 // Warp roles: warp 0 issues the tensor-map copies (128 bytes of the reduction of both
 // operands per stage, 128-byte swizzle), warp 1 allocates tensor memory and issues the
@@ -148,7 +147,7 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 // Arrive on a barrier given by its cluster address (own or peer CTA), with the default
 // semantics: what these arrivals order are tensor-map copies and tensor-memory reads,
 // which complete before them. (At cluster scope an arrival waits for the warp's output
-// stores and every wait reloads the L1: 8192 x 4096 x 4096 took 548 us instead of 299.)
+// stores and every wait reloads the L1: 8192 x 4096 x 4096 took 548 us instead of 297.)
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr)
                  : "memory");
@@ -346,8 +345,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t tmem = tmem_base;
 
     // The copying and the multiplying warp run their loops whole and one elected lane
-    // issues: with operands in uniform registers an MMA costs its issuer a few clocks,
-    // from a loop of one lane it cost 100 (and the kernel half of its speed).
+    // issues: with warp-uniform operands a stage of four MMAs costs its issuer 390 clocks,
+    // less than the 512 that they take; from a loop of one lane it cost 700, and
+    // 8192 x 4096 x 4096 took 297 us instead of 257.
     if (warp == 0) {
         const bool lead = elect_one();
         Ring<kPairStages> ring;
@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
         if (reader && ok) {
             // this CTA adds the columns [c0, c1), kWide at a time; the loads of two CTAs
             // are in flight together
-            constexpr int kWide = BN >= 64 ? 8 : 2;
+            constexpr int kWide = BN / 8;
             const int c0 = share(BN, rank, ctas), c1 = share(BN, rank + 1, ctas);
             const uint32_t at0 = smem_u32(&sums[ch]);
             for (int c = c0; c < c1; c += kWide) {
@@ -805,17 +805,18 @@ bool encode(CUtensorMap* map, const void* p, int64_t rows, int64_t K, int64_t ld
 }
 
 // Which kernel, and how a tile of the split kernel is cut. Measured with cold inputs,
-// us with about 5 us of the measurement itself:
-//   pairs from 96 tiles of 128 x 128 on (32 pairs at work): 1024 x 2048 by K = 512 18
-//     against 26 split, 512 x 4096 by 1024 23 against 33; below, fewer pairs lose:
-//     2048 x 512 by 2048 32 against 29, 8192 x 128 by 512 20 against 17.
-//   BN: the narrowest tile that leaves at least three quarters of the SMs to the
-//     reduction's shares: 64 x 4096 by 4096 29 (64 columns, 4 shares) against 34 (16
-//     columns, 2 shares); 33 x 1000 by 1000 14 (16 columns, 4 shares) against 19 (64).
-//   shares: as many as the SMs hold, 4 blocks of the reduction each or more: 1 x 512
-//     by 2048 14 with 8, 25 with 1; 16 x 4096 by 4096 25 against 43. The exchange costs
-//     2 us (16 columns) to 4 us (64), so short reductions are not shared: 16 x 512 by
-//     512 13 whole, 14 in two; 256 x 1024 by 1024 20 whole, 21 in two or four.
+// us with about 4 us of the measurement itself:
+//   pairs from 96 tiles of 128 x 128 on (32 pairs at work): 1536 x 1024 by K = 512 16
+//     against 20 split, 512 x 4096 by 1024 20 against 31; below, fewer pairs win nothing or
+//     lose: 512 x 2048 by 2048 27 against 27, 8192 x 128 by 512 18 against 14.
+//   BN: 16 while that leaves the reduction four shares or more, else 32, so that the
+//     weights are read fewer times: 64 x 4096 by 4096 25 (32 columns, 4 shares) against 31
+//     (16, 2 shares); 33 x 1000 by 1000 12 (16 columns) against 14 (32). 64 columns were
+//     never faster.
+//   shares: up to two CTAs per SM, 3 blocks of the reduction each or more: 1 x 512 by
+//     2048 12 with 8, 23 with 1; 16 x 512 by 512 10 with 4, 12 with 1. The exchange of 32
+//     columns wants 10 blocks: 128 x 4096 by 4096 33 with 2, 41 with 1; 700 x 700 by 700
+//     16 with 2, 14 with 1.
 struct Route {
     bool pair;
     int bn, ctas;
@@ -823,11 +824,11 @@ struct Route {
 Route route(int64_t M, int64_t N, int64_t K) {
     const int64_t items = 3 * ((K + kBK - 1) / kBK), ntiles = (N + 127) / 128;
     if (((M + 127) / 128) * ntiles >= 96) return {true, 256, 2};
-    Route r{false, 16, 1};
-    while (r.bn < 64 && ((M + r.bn - 1) / r.bn) * ntiles > kNumSMs / 4) r.bn *= 2;
+    Route r{false, ((M + 15) / 16) * ntiles <= kNumSMs / 4 ? 16 : 32, 1};
     const int64_t tiles = ((M + r.bn - 1) / r.bn) * ntiles;
-    if (items >= (r.bn == 64 ? 36 : 18))
-        while (r.ctas < 8 && tiles * r.ctas * 2 <= kNumSMs && items >= r.ctas * 8) r.ctas *= 2;
+    const int64_t least = r.bn == 16 ? 3 : 10;
+    while (r.ctas < 8 && tiles * r.ctas * 2 <= kNumSMs * 2 && items >= r.ctas * 2 * least)
+        r.ctas *= 2;
     return r;
 }
 
@@ -931,6 +932,5 @@ extern "C" int tagi_int8_moment_matmul(const int8_t* x_m, const uint8_t* x_2, co
     cudaStream_t st = as_stream(stream);
     if (r.pair) return launch_pair(g, maps, st, what);
     if (r.bn == 16) return launch_split<16>(g, maps, r.ctas, st, what);
-    if (r.bn == 32) return launch_split<32>(g, maps, r.ctas, st, what);
-    return launch_split<64>(g, maps, r.ctas, st, what);
+    return launch_split<32>(g, maps, r.ctas, st, what);
 }
