@@ -461,13 +461,43 @@ __global__ void values_kernel(const NormArgs g, float* vm, float* v2, float* vS)
 // Both are formed in one pass: block (slice, columns) walks its rows with its columns'
 // sums in registers, kBackThreads / x rows at a time (x threads along the columns), adds
 // the groups' sums in order and leaves them in the workspace; a second launch adds the
-// slices in order and applies them. Bound by HBM: 28 bytes per element. 16384 x 512:
+// slices in order and applies them (a single slice applies its own). Bound by HBM: 28 bytes per element. 16384 x 512:
 // 43.6 us with the second launch, 5.4 TB/s; without the row groups there were four times
 // the slices and the second launch alone took 15 us.
 constexpr int kBackThreads = 512;
 constexpr int kBackCols = 128;  // threads along the columns, at most
 
+// What becomes of gamma's sums.
+struct GammaOut {
+    int mode;
+    double* sums;
+    float* w;
+    float* Sw;
+    float* d_w;
+    float* d_Sw;
+    float cap;
+};
+__device__ __forceinline__ void gamma_out(const GammaOut& o, int j, int ni, double a, double b) {
+    if (o.mode == TAGI_WGRAD_SUMS) {
+        o.sums[j] = a;
+        o.sums[ni + j] = b;
+        return;
+    }
+    const float S = o.Sw[j];
+    const float dm = static_cast<float>(a) * S, dS = static_cast<float>(b) * S * S;
+    if (o.mode == TAGI_WGRAD_DELTAS) {
+        o.d_w[j] = dm;
+        o.d_Sw[j] = dS;
+        return;
+    }
+    float m = o.w[j], v = S;
+    capped_pair(m, v, dm, dS, o.cap);
+    o.w[j] = m;
+    o.Sw[j] = v;
+}
+
 struct BackArgs {
+    GammaOut gamma;  // used here when one slice holds all rows
     const float* dm;
     const float* dS;
     const float* h;
@@ -531,24 +561,30 @@ __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackArgs g) {
         red[1][at + e] = sS[e];
     }
     __syncthreads();
-    // a thread per column and sum
+    // a thread per column
     const int cols = blockDim.x * VEC;
-    for (int i = grp * blockDim.x + threadIdx.x; i < 2 * cols; i += kBackThreads) {
-        const int which = i / cols, c = i - which * cols;
+    for (int c = grp * blockDim.x + threadIdx.x; c < cols; c += kBackThreads) {
         const int col = blockIdx.y * cols + c;
         if (col >= g.ni) continue;
-        double a = red[which][c];
-        for (int k = 1; k < groups; ++k) a += red[which][k * cols + c];
-        g.part[(static_cast<int64_t>(blockIdx.x) * 2 + which) * g.ni + col] = a;
+        double a = red[0][c], b = red[1][c];
+        for (int k = 1; k < groups; ++k) {
+            a += red[0][k * cols + c];
+            b += red[1][k * cols + c];
+        }
+        if (gridDim.x == 1) {
+            gamma_out(g.gamma, col, g.ni, a, b);
+            continue;
+        }
+        double* p = g.part + static_cast<int64_t>(blockIdx.x) * 2 * g.ni + col;
+        p[0] = a;
+        p[g.ni] = b;
     }
 }
 
 // Adds the slices' sums: 8 columns per block, 32 threads per column, each every 32nd
 // slice (a fixed order), their sums by a shuffle tree of fixed shape.
 __global__ void __launch_bounds__(256) back_finish_kernel(const double* part, int slices, int ni,
-                                                          int mode, double* sums, float* w,
-                                                          float* Sw, float* d_w, float* d_Sw,
-                                                          float cap) {
+                                                          const GammaOut out) {
     __shared__ double red[2][8][33];
     const int c = threadIdx.x & 7, g = threadIdx.x >> 3;
     const int col = blockIdx.x * 8 + c;
@@ -573,23 +609,7 @@ __global__ void __launch_bounds__(256) back_finish_kernel(const double* part, in
         b += __shfl_xor_sync(0xffffffffu, b, o);
     }
     const int j = blockIdx.x * 8 + warp;
-    if (lane != 0 || j >= ni) return;
-    if (mode == TAGI_WGRAD_SUMS) {
-        sums[j] = a;
-        sums[ni + j] = b;
-        return;
-    }
-    const float S = Sw[j];
-    const float dm = static_cast<float>(a) * S, dS = static_cast<float>(b) * S * S;
-    if (mode == TAGI_WGRAD_DELTAS) {
-        d_w[j] = dm;
-        d_Sw[j] = dS;
-        return;
-    }
-    float m = w[j], v = S;
-    capped_pair(m, v, dm, dS, cap);
-    w[j] = m;
-    Sw[j] = v;
+    if (lane == 0 && j < ni) gamma_out(out, j, ni, a, b);
 }
 
 // Threads along the columns of `vecs` vectors, and slices of rows: three blocks per SM
@@ -738,6 +758,7 @@ extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, con
     BackArgs g{};
     g.dm = dmz; g.dS = dSz; g.h = hm; g.inv = inv_rms; g.w = mw; g.rm = rm; g.rS = rS;
     g.om = d_m; g.oS = d_S; g.part = static_cast<double*>(workspace);
+    g.gamma = {mode, sums, mw, Sw, d_mw, d_Sw, cap_factor};
     g.rows = rows; g.ni = static_cast<int>(ni);
     uintptr_t bits = 0;
     for (const void* p : {static_cast<const void*>(dmz), static_cast<const void*>(dSz),
@@ -759,9 +780,8 @@ extern "C" int tagi_add_rmsnorm_backward(const float* dmz, const float* dSz, con
     else
         launch_early(back_kernel<1>, {grid, block, st}, g);
     const int rc = check_launch(what);
-    if (rc) return rc;
+    if (rc || slices == 1) return rc;
     launch_early(back_finish_kernel, {dim3(static_cast<unsigned>((ni + 7) / 8)), dim3(256), st},
-                 static_cast<const double*>(g.part), slices, g.ni, mode, sums, mw, Sw, d_mw, d_Sw,
-                 cap_factor);
+                 static_cast<const double*>(g.part), slices, g.ni, g.gamma);
     return check_launch(what);
 }

@@ -19,7 +19,7 @@ import torch
 from torch import Tensor
 
 from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on,
-                    empty_on, lib, ptr, workspace)
+                    empty_on, lib, ptr)
 
 _ID_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
@@ -64,9 +64,11 @@ def _grad(mode, ids, dmz, dSz, V, D, scale, padding_idx, mw, Sw, out_m, out_S, c
         raise ValueError(f"deltas {tuple(dmz.shape)} and {tuple(dSz.shape)} do not match "
                          f"{n} tokens of {D} columns")
     ids, dmz, dSz = ids.contiguous(), dmz.contiguous(), dSz.contiguous()
-    hold, wp, wn = workspace(lib().size("tagi_embedding_grad_workspace_size", n, D), dmz)
+    wn = lib().size("tagi_embedding_grad_workspace_size", n, D)
+    hold = empty_on(dev, (wn,), (1,), torch.uint8)
     call_on(dev, "tagi_embedding_grad", ids.data_ptr(), code, dmz.data_ptr(), dSz.data_ptr(), n,
-            V, D, padding_idx, scale, mode, ptr(mw), ptr(Sw), ptr(out_m), ptr(out_S), cap, wp, wn)
+            V, D, padding_idx, scale, mode, ptr(mw), ptr(Sw), ptr(out_m), ptr(out_S), cap,
+            hold.data_ptr(), wn)
 
 
 def embedding_grad(ids: Tensor, dmz: Tensor, dSz: Tensor, num_embeddings: int, scale: float = 1.0,
@@ -83,8 +85,9 @@ def embedding_grad(ids: Tensor, dmz: Tensor, dSz: Tensor, num_embeddings: int, s
             raise ValueError(f"Sw {tuple(Sw.shape)} is not ({num_embeddings}, {D})")
         Sw = Sw.contiguous()
     if out is None:
-        g_m = dmz.new_empty((num_embeddings, D))
-        g_S = torch.empty_like(g_m)
+        dev = check_f32(dmz)
+        g_m = empty_on(dev, (num_embeddings, D), (D, 1))
+        g_S = empty_on(dev, (num_embeddings, D), (D, 1))
     else:
         g_m, g_S = out
         for t in out:

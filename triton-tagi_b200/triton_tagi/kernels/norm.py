@@ -13,7 +13,7 @@ import torch
 from torch import Tensor
 
 from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on,
-                    empty_on, lib, ptr, workspace)
+                    empty_on, lib, ptr)
 from .int8 import Int8Moments, _pointers, empty_codes
 
 
@@ -90,11 +90,12 @@ def _backward(mode, dmz, dSz, hm, inv, mw, Sw, rm, rS, sums=None, d_mw=None, d_S
     dmz, dSz, hm, inv, rm, rS = _cont(dmz, dSz, hm, inv, rm, rS)
     size, stride = tuple(dmz.shape), dmz.stride()
     d_m, d_S = empty_on(dev, size, stride), empty_on(dev, size, stride)
-    hold, wp, wn = workspace(lib().size("tagi_add_rmsnorm_backward_workspace_size", rows, width),
-                             dmz)
+    wn = lib().size("tagi_add_rmsnorm_backward_workspace_size", rows, width)
+    hold = empty_on(dev, (wn,), (1,), torch.uint8)
     call_on(dev, "tagi_add_rmsnorm_backward", dmz.data_ptr(), dSz.data_ptr(), hm.data_ptr(),
             inv.data_ptr(), ptr(rm), ptr(rS), d_m.data_ptr(), d_S.data_ptr(), mode, ptr(sums),
-            mw.data_ptr(), ptr(Sw), ptr(d_mw), ptr(d_Sw), cap, rows, width, wp, wn)
+            mw.data_ptr(), ptr(Sw), ptr(d_mw), ptr(d_Sw), cap, rows, width,
+            hold.data_ptr(), wn)
     return d_m, d_S
 
 
@@ -104,8 +105,10 @@ def add_rmsnorm_backward(dmz: Tensor, dSz: Tensor, hm: Tensor, inv: Tensor, mw: 
     inv μ_γ δμ_z + δμ_h and (inv μ_γ)² δS_z + δS_h with the deltas (rm, rS) that reach
     the stream behind the norm (None: none), and the deltas of the scale parameters,
     S_γ Σ inv μ_h δμ_z and S_γ² Σ (inv μ_h)² δS_z."""
+    _pair("add_rmsnorm_backward", rm, rS)
     mw, Sw = _cont(mw, Sw)
-    d_mw, d_Sw = torch.empty_like(mw), torch.empty_like(Sw)
+    dev, size, stride = check_f32(mw, Sw), tuple(mw.shape), mw.stride()
+    d_mw, d_Sw = empty_on(dev, size, stride), empty_on(dev, size, stride)
     d_m, d_S = _backward(WGRAD_DELTAS, dmz, dSz, hm, inv, mw, Sw, rm, rS, d_mw=d_mw, d_Sw=d_Sw)
     return d_m, d_S, d_mw, d_Sw
 
