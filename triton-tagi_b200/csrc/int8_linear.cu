@@ -587,6 +587,8 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
         abort_flag = give_up;
         if (give_up) atomicCAS(&g_int8_error, 0, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // this thread's copies use the barriers before any synchronisation of the CTA
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         // the first stages fill while the others set up
         wait_for_primary();
         for (; !give_up && issued < end && issued < beg + P::STAGES; ++issued) issue(issued, issued - beg);

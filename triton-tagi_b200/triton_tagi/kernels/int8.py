@@ -103,10 +103,11 @@ def _quantize(m: Tensor, S: Tensor, weights: bool) -> Int8Moments:
         raise ValueError(f"means {tuple(m.shape)} and variances {tuple(S.shape)} must have one "
                          "shape and a last dimension")
     width = m.shape[-1]
-    m, S = m.reshape(-1, width).contiguous(), S.reshape(-1, width).contiguous()
-    q = empty_codes(m.shape[0], width, dev)
+    rows = m.numel() // width
+    m, S = m.contiguous(), S.contiguous()
+    q = empty_codes(rows, width, dev)
     call_on(dev, "tagi_quantize_moments", m.data_ptr(), S.data_ptr(), 1 if weights else 0,
-            *_pointers(q, width), m.shape[0], width)
+            *_pointers(q, width), rows, width)
     return q
 
 
