@@ -177,6 +177,61 @@ def test_empty_batch_of_tokens():
     assert (mw == 1).all() and (Sw == 1).all()
 
 
+def test_gradient_against_differences():
+    """The lookup is linear in the table, so a difference of its outputs along one entry,
+    weighted with the deltas, is that entry's sum; variances enter with the scale squared."""
+    from triton_tagi.kernels import embedding_grad, embedding_lookup
+
+    g = gen(31)
+    V, D, n, s = 12, 5, 90, 1.5
+    ids = torch.randint(0, V, (n,), device=DEV, generator=g)
+    mw, Sw = randn(g, V, D), rand(g, V, D)
+    dm, dS = randn(g, n, D), -rand(g, n, D)
+    g_m, g_S = embedding_grad(ids, dm, dS, V, scale=s, padding_idx=3)
+    for v, j in ((0, 0), (3, 1), (7, 4), (11, 2)):
+        up = [t.clone() for t in (mw, Sw)]
+        for t in up:
+            t[v, j] = 0.0
+        lo = embedding_lookup(ids, *up, scale=s, padding_idx=3)
+        for t in up:
+            t[v, j] = 1.0
+        hi = embedding_lookup(ids, *up, scale=s, padding_idx=3)
+        for a, b, d, got in ((hi[0], lo[0], dm, g_m), (hi[1], lo[1], dS, g_S)):
+            diff = (a.double() - b.double()) * d.double()
+            assert abs(got[v, j].item() - diff.sum().item()) <= 34 * U * diff.abs().sum().item()
+
+
+def test_strided_operands():
+    """Views with other strides give what their contiguous copies give."""
+    from triton_tagi import kernels as K
+
+    g = gen(32)
+    wide = [randn(g, 48, 60) for _ in range(4)]
+    a = [t[::2, ::3].t() for t in wide]  # 20 x 24
+    a[1], a[3] = a[1].abs(), a[3].abs()
+    c = [t.contiguous() for t in a]
+    w, Sw = rand(g, 48)[::2] + 0.5, rand(g, 24)
+    for f in (K.add_rmsnorm, K.add_rmsnorm_int8):
+        x, y = f(*a, w, Sw), f(*c, w.contiguous(), Sw)
+        for p, q in zip(x, y):
+            for u, v in zip(p, q) if isinstance(p, tuple) else ((p, q),):
+                assert torch.equal(u, v)
+    inv = rand(g, 40)[::2] + 0.5
+    x = K.add_rmsnorm_backward(a[0], a[1], a[2], inv, w, Sw, a[3], a[0])
+    y = K.add_rmsnorm_backward(c[0], c[1], c[2], inv.contiguous(), w.contiguous(), Sw, c[3], c[0])
+    assert all(torch.equal(u, v) for u, v in zip(x, y))
+    for f in (K.quantize_moments, K.quantize_weights):
+        assert all(torch.equal(u, v) for u, v in zip(f(a[0], a[1]), f(c[0], c[1])))
+    ids = torch.randint(0, 20, (30, 2), device=DEV, generator=g)[:, 0]
+    x, y = K.embedding_lookup(ids, a[0], a[1]), K.embedding_lookup(ids.contiguous(), c[0], c[1])
+    assert all(torch.equal(u, v) for u, v in zip(x, y))
+    d = randn(g, 24, 30).t()
+    x, y = K.embedding_grad(ids, d, -d, 20), K.embedding_grad(ids.contiguous(), d.contiguous(), -d, 20)
+    assert all(torch.equal(u, v) for u, v in zip(x, y))
+    with pytest.raises(ValueError, match="contiguous"):
+        K.embedding_update(ids, d, d, a[0], a[1], 2.0)
+
+
 def test_update_of_deltas_that_are_not_numbers():
     """As update_parameters: a NaN delta leaves its parameter, an infinite one moves it by
     the cap."""
