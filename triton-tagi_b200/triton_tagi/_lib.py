@@ -263,11 +263,14 @@ def call_on(dev: int, name: str, *args) -> None:
             L.fail(name, rc)
 
 
-def empty_on(dev: int, size, stride, dtype=torch.float32) -> torch.Tensor:
-    """An uninitialised tensor of the given strides on CUDA device ``dev``."""
+def allocator(dev: int):
+    """``new(size, stride, dtype)``: uninitialised tensors on CUDA device ``dev``; size and
+    stride are tuples of integers."""
     if _fast_empty is not None and dev == _current_device():
-        return _fast_empty(size, stride, dtype)
-    return torch.empty_strided(size, stride, dtype=dtype, device=torch.device("cuda", dev))
+        return _fast_empty
+    device = torch.device("cuda", dev)
+    return lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype,
+                                                           device=device)
 
 
 def workspace(nbytes: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int | None, int]:

@@ -18,8 +18,8 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on,
-                    empty_on, lib, ptr)
+from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, allocator, call_on, check_f32,
+                    check_on, lib, ptr)
 
 _ID_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
@@ -47,7 +47,8 @@ def embedding_lookup(ids: Tensor, mw: Tensor, Sw: Tensor, scale: float = 1.0,
     V, D = _check_table(mw, Sw)
     ids, mw, Sw = ids.contiguous(), mw.contiguous(), Sw.contiguous()
     n, shape = ids.numel(), ids.shape
-    mz, Sz = empty_on(dev, (n, D), (D, 1)), empty_on(dev, (n, D), (D, 1))
+    new = allocator(dev)
+    mz, Sz = new((n, D), (D, 1), torch.float32), new((n, D), (D, 1), torch.float32)
     call_on(dev, "tagi_embedding_lookup", ids.data_ptr(), code, mw.data_ptr(), Sw.data_ptr(),
             mz.data_ptr(), Sz.data_ptr(), n, V, D, padding_idx, scale)
     if len(shape) != 1:
@@ -65,7 +66,7 @@ def _grad(mode, ids, dmz, dSz, V, D, scale, padding_idx, mw, Sw, out_m, out_S, c
                          f"{n} tokens of {D} columns")
     ids, dmz, dSz = ids.contiguous(), dmz.contiguous(), dSz.contiguous()
     wn = lib().size("tagi_embedding_grad_workspace_size", n, D)
-    hold = empty_on(dev, (wn,), (1,), torch.uint8)
+    hold = allocator(dev)((wn,), (1,), torch.uint8)
     call_on(dev, "tagi_embedding_grad", ids.data_ptr(), code, dmz.data_ptr(), dSz.data_ptr(), n,
             V, D, padding_idx, scale, mode, ptr(mw), ptr(Sw), ptr(out_m), ptr(out_S), cap,
             hold.data_ptr(), wn)
@@ -85,9 +86,8 @@ def embedding_grad(ids: Tensor, dmz: Tensor, dSz: Tensor, num_embeddings: int, s
             raise ValueError(f"Sw {tuple(Sw.shape)} is not ({num_embeddings}, {D})")
         Sw = Sw.contiguous()
     if out is None:
-        dev = check_f32(dmz)
-        g_m = empty_on(dev, (num_embeddings, D), (D, 1))
-        g_S = empty_on(dev, (num_embeddings, D), (D, 1))
+        new, size = allocator(check_f32(dmz)), (int(num_embeddings), D)
+        g_m, g_S = new(size, (D, 1), torch.float32), new(size, (D, 1), torch.float32)
     else:
         g_m, g_S = out
         for t in out:

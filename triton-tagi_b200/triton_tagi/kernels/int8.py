@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 from torch import Tensor
 
-from .._lib import call_on, check_f32, check_on, empty_on, ptr
+from .._lib import allocator, call_on, check_f32, check_on, ptr
 
 
 class Int8Moments(NamedTuple):
@@ -38,9 +38,8 @@ class Int8Moments(NamedTuple):
         """What the codes stand for: three float32 ``(rows, width)`` tensors."""
         dev = check_f32(self.scales)
         pointers, rows, width, _hold = _checked(self, dev)
-        size, stride = (rows, width), (width, 1)
-        v_m, v_2, v_S = (empty_on(dev, size, stride), empty_on(dev, size, stride),
-                         empty_on(dev, size, stride))
+        new, size, stride, f32 = allocator(dev), (rows, width), (width, 1), torch.float32
+        v_m, v_2, v_S = new(size, stride, f32), new(size, stride, f32), new(size, stride, f32)
         call_on(dev, "tagi_int8_values", *pointers, v_m.data_ptr(), v_2.data_ptr(), v_S.data_ptr(),
                 rows, width)
         return v_m, v_2, v_S
@@ -49,11 +48,9 @@ class Int8Moments(NamedTuple):
 def empty_codes(rows: int, width: int, dev: int) -> Int8Moments:
     """Uninitialised codes whose rows start on 16-byte boundaries, as the tensor-core
     product's copies need them."""
-    size, stride = (rows, width), ((width + 15) // 16 * 16, 1)
-    return Int8Moments(empty_on(dev, size, stride, torch.int8),
-                       empty_on(dev, size, stride, torch.uint8),
-                       empty_on(dev, size, stride, torch.uint8),
-                       empty_on(dev, (3, rows), (rows, 1)))
+    new, size, stride = allocator(dev), (rows, width), ((width + 15) // 16 * 16, 1)
+    return Int8Moments(new(size, stride, torch.int8), new(size, stride, torch.uint8),
+                       new(size, stride, torch.uint8), new((3, rows), (rows, 1), torch.float32))
 
 
 def _checked(q: Int8Moments, dev: int) -> tuple:
@@ -137,7 +134,8 @@ def int8_moments_matmul(x: Int8Moments, w: Int8Moments, mb: Tensor | None = None
         raise ValueError(f"biases must hold {N} values")
     mb = None if mb is None else mb.contiguous()
     Sb = None if Sb is None else Sb.contiguous()
-    mz, Sz = empty_on(dev, (M, N), (N, 1)), empty_on(dev, (M, N), (N, 1))
+    new = allocator(dev)
+    mz, Sz = new((M, N), (N, 1), torch.float32), new((M, N), (N, 1), torch.float32)
     call_on(dev, "tagi_int8_moment_matmul", *px, *pw, ptr(mb), ptr(Sb),
             mz.data_ptr(), Sz.data_ptr(), M, N, K)
     return mz, Sz

@@ -12,8 +12,8 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, call_on, check_f32, check_on,
-                    empty_on, lib, ptr)
+from .._lib import (WGRAD_DELTAS, WGRAD_SUMS, WGRAD_UPDATE, allocator, call_on, check_f32,
+                    check_on, lib, ptr)
 from .int8 import Int8Moments, _pointers, empty_codes
 
 
@@ -51,10 +51,10 @@ def add_rmsnorm(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | None, mw
     _pair("add_rmsnorm", mr, Sr)
     dev, rows, width = _rows("add_rmsnorm", mw, Sw, ma, Sa, mr, Sr)
     ma, Sa, mr, Sr, mw, Sw = _cont(ma, Sa, mr, Sr, mw, Sw)
-    size, stride = tuple(ma.shape), ma.stride()
-    hm, hS = (ma, Sa) if mr is None else (empty_on(dev, size, stride), empty_on(dev, size, stride))
-    mz, Sz = empty_on(dev, size, stride), empty_on(dev, size, stride)
-    inv = empty_on(dev, (rows,), (1,))
+    new, size, stride, f32 = allocator(dev), tuple(ma.shape), ma.stride(), torch.float32
+    hm, hS = (ma, Sa) if mr is None else (new(size, stride, f32), new(size, stride, f32))
+    mz, Sz = new(size, stride, f32), new(size, stride, f32)
+    inv = new((rows,), (1,), f32)
     if len(size) != 2:
         inv = inv.view(size[:-1])
     call_on(dev, "tagi_add_rmsnorm_forward", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
@@ -70,8 +70,10 @@ def add_rmsnorm_int8(ma: Tensor, Sa: Tensor, mr: Tensor | None, Sr: Tensor | Non
     _pair("add_rmsnorm_int8", mr, Sr)
     dev, rows, width = _rows("add_rmsnorm_int8", mw, Sw, ma, Sa, mr, Sr)
     ma, Sa, mr, Sr, mw, Sw = _cont(ma, Sa, mr, Sr, mw, Sw)
-    size, stride = tuple(ma.shape), ma.stride()
-    hm, hS = (ma, Sa) if mr is None else (empty_on(dev, size, stride), empty_on(dev, size, stride))
+    hm, hS = ma, Sa
+    if mr is not None:
+        new, size, stride, f32 = allocator(dev), tuple(ma.shape), ma.stride(), torch.float32
+        hm, hS = new(size, stride, f32), new(size, stride, f32)
     q = empty_codes(rows, width, dev)
     call_on(dev, "tagi_add_rmsnorm_int8", ma.data_ptr(), Sa.data_ptr(), ptr(mr), ptr(Sr),
             mw.data_ptr(), Sw.data_ptr(), hm.data_ptr(), hS.data_ptr(), *_pointers(q, width), rows,
@@ -88,10 +90,10 @@ def _backward(mode, dmz, dSz, hm, inv, mw, Sw, rm, rS, sums=None, d_mw=None, d_S
         raise ValueError(f"{name}: the stream {tuple(hm.shape)} and 1/rms {tuple(inv.shape)} do "
                          f"not match {rows} rows of {width}")
     dmz, dSz, hm, inv, rm, rS = _cont(dmz, dSz, hm, inv, rm, rS)
-    size, stride = tuple(dmz.shape), dmz.stride()
-    d_m, d_S = empty_on(dev, size, stride), empty_on(dev, size, stride)
+    new, size, stride, f32 = allocator(dev), tuple(dmz.shape), dmz.stride(), torch.float32
+    d_m, d_S = new(size, stride, f32), new(size, stride, f32)
     wn = lib().size("tagi_add_rmsnorm_backward_workspace_size", rows, width)
-    hold = empty_on(dev, (wn,), (1,), torch.uint8)
+    hold = new((wn,), (1,), torch.uint8)
     call_on(dev, "tagi_add_rmsnorm_backward", dmz.data_ptr(), dSz.data_ptr(), hm.data_ptr(),
             inv.data_ptr(), ptr(rm), ptr(rS), d_m.data_ptr(), d_S.data_ptr(), mode, ptr(sums),
             mw.data_ptr(), ptr(Sw), ptr(d_mw), ptr(d_Sw), cap, rows, width,
@@ -107,8 +109,8 @@ def add_rmsnorm_backward(dmz: Tensor, dSz: Tensor, hm: Tensor, inv: Tensor, mw: 
     S_γ Σ inv μ_h δμ_z and S_γ² Σ (inv μ_h)² δS_z."""
     _pair("add_rmsnorm_backward", rm, rS)
     mw, Sw = _cont(mw, Sw)
-    dev, size, stride = check_f32(mw, Sw), tuple(mw.shape), mw.stride()
-    d_mw, d_Sw = empty_on(dev, size, stride), empty_on(dev, size, stride)
+    new, size, stride = allocator(check_f32(mw, Sw)), tuple(mw.shape), mw.stride()
+    d_mw, d_Sw = new(size, stride, torch.float32), new(size, stride, torch.float32)
     d_m, d_S = _backward(WGRAD_DELTAS, dmz, dSz, hm, inv, mw, Sw, rm, rS, d_mw=d_mw, d_Sw=d_Sw)
     return d_m, d_S, d_mw, d_Sw
 
