@@ -1,0 +1,90 @@
+"""Token-path operators, further cases: 8-bit products on the CTA-pair route, operators
+beside other work on the device, rows of every width class, scales whose squares are not
+exact, and what a served network leaves alone.
+
+Tolerances count roundings of u = 2^-24 (half a float32 step, relative), as in
+test_gpu_token_path.py, whose plain float64 forms these tests share.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_token_path import DEV, U, gen, operand, plain_linear, rand, randn, within
+
+pytestmark = pytest.mark.gpu
+
+
+# -- the CTA-pair route of the 8-bit product ----------------------------------------------
+# 96 or more tiles of 128 x 128; a pair computes 256 x 256 and there are 74 of them.
+
+PAIRS = [
+    # M, N, K
+    (3333, 3001, 129),   # 14 x 12 tiles of 256: two and three per pair, all edges ragged
+    (5000, 2570, 640),   # 20 x 11: the last channels are 10 of a pair's first CTA alone
+    (257, 12300, 40),    # 2 x 49: one token in the last tile; the reduction ends in its block
+    (12289, 127, 1),     # 49 x 1: no channel for the second CTA; a reduction of one
+    (1536, 1024, 512),   # 6 x 4: no edge at all, fewer tiles than pairs
+    (2050, 2305, 1030),  # 9 x 10: more than one round of stages per product
+]
+
+
+@pytest.mark.parametrize("M,N,K", PAIRS)
+@pytest.mark.parametrize("bias", [True, False])
+def test_int8_moments_matmul_by_pairs(M, N, K, bias):
+    """Against the float64 form, over all rows. The sums are exact; each is converted (1
+    rounding) and scaled by its token (1); the channel's scale and the bias take 1 on the
+    result, and the variance's first product with the bias 1 on a part of it."""
+    from triton_tagi._lib import device_status
+    from triton_tagi.kernels import int8_moments_matmul
+
+    assert ((M + 127) // 128) * ((N + 127) // 128) >= 96
+    g = gen(M + N + K)
+    x, w = operand(g, M, K), operand(g, N, K)
+    mb, Sb = (randn(g, N), rand(g, N)) if bias else (None, None)
+    mz, Sz = int8_moments_matmul(x, w, mb, Sb)
+    rm, rS, tm, tS = plain_linear(x, w, mb, Sb)
+    within(mz, rm, U * (4 * tm + rm.abs()), "mz")
+    within(Sz, rS, U * (4 * tS + 2 * rS.abs()), "Sz")
+    again = int8_moments_matmul(x, w, mb, Sb)
+    assert torch.equal(mz, again[0]) and torch.equal(Sz, again[1])
+    assert device_status() == 0
+
+
+def test_rows_by_pairs_that_are_not_finite_stay_alone():
+    """Scales that are NaN make their own token NaN and no other, in every tile of a pair."""
+    from triton_tagi.kernels import int8_moments_matmul
+
+    g = gen(41)
+    x, w = operand(g, 3333, 129), operand(g, 3001, 129)
+    bad = torch.zeros(3333, dtype=torch.bool, device=DEV)
+    bad[[0, 255, 256, 1999, 3332]] = True
+    x.scales[:, bad] = float("nan")
+    mz, Sz = int8_moments_matmul(x, w)
+    assert torch.equal(mz.isnan().all(1), bad) and torch.equal(mz.isnan().any(1), bad)
+    assert torch.equal(Sz.isnan().all(1), bad) and torch.equal(Sz.isnan().any(1), bad)
+
+
+def test_the_abort_path_of_pairs_releases_its_memory_and_reports():
+    """As test_the_abort_path_releases_its_memory_and_reports, with several tiles per pair:
+    the host's limit makes both CTAs of every pair give up before their first stage."""
+    from triton_tagi._lib import device_status, set_wait_limit_ns
+    from triton_tagi.kernels import int8_moments_matmul
+
+    g = gen(42)
+    x, w = operand(g, 3333, 640), operand(g, 3001, 640)
+    ref = int8_moments_matmul(x, w)
+    assert device_status(reset=True) == 0
+    set_wait_limit_ns(500)
+    try:
+        int8_moments_matmul(x, w)
+        torch.cuda.synchronize()
+    finally:
+        set_wait_limit_ns(0)
+    assert device_status(reset=True) != 0
+    assert device_status() == 0
+    for _ in range(2):
+        got = int8_moments_matmul(x, w)
+        assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+    assert device_status() == 0

@@ -85,14 +85,26 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count)
                  : "memory");
 }
+// Scopes of a wait: CTA for arrivals of this CTA's threads, copies and MMAs; CLUSTER where
+// the other CTA's threads arrive (arrive_landed, arrive_read).
+enum { CTA = 0, CLUSTER = 1 };
+template <int SCOPE = CTA>
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
-        : "memory");
+    if (SCOPE == CLUSTER)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, "
+            "[%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+            : "memory");
     return ok != 0;
 }
 struct Abort {
@@ -100,12 +112,13 @@ struct Abort {
     uint32_t peer;       // cluster address of the peer CTA's (0: none)
 };
 // False if the CTA gave up, or if this wait ran out (it and its peer then give up).
+template <int SCOPE>
 __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, const Abort& ab,
                                             int code) {
     const unsigned long long t0 = globaltimer();
     const unsigned long long limit = *const_cast<volatile unsigned long long*>(&g_int8_wait_ns);
     for (;;) {
-        if (mbar_try(bar, parity)) return true;
+        if (mbar_try<SCOPE>(bar, parity)) return true;
         if (*ab.flag) return false;
         if (globaltimer() - t0 > limit) {
             *ab.flag = 1;
@@ -116,14 +129,16 @@ __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, cons
         }
     }
 }
+template <int SCOPE = CTA>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const Abort& ab,
                                           int code) {
-    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, ab, code);
+    return mbar_try<SCOPE>(bar, parity) || mbar_wait_slow<SCOPE>(bar, parity, ab, code);
 }
 // The same for a whole warp, so that what follows stays uniform.
+template <int SCOPE = CTA>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab,
                                           int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, code));
+    return __all_sync(0xffffffffu, mbar_wait<SCOPE>(bar, parity, ab, code));
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -144,12 +159,22 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
                  "r"(bytes)
                  : "memory");
 }
-// Arrive on a barrier given by its cluster address (own or peer CTA), with the default
-// semantics: what these arrivals order are tensor-map copies and tensor-memory reads,
-// which complete before them. (At cluster scope an arrival waits for the warp's output
-// stores and every wait reloads the L1: 8192 x 4096 x 4096 took 548 us instead of 297.)
-__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr)
+// Arrive on a barrier given by its cluster address (own or peer CTA). Two kinds, for what
+// the other CTA's multiplying warp does behind its wait (an acquire at cluster scope):
+//   landed  publishes what this warp has seen: a stage that has landed in this CTA's shared
+//           memory, which the MMAs of the pair's first CTA read. The release covers shared
+//           memory alone: one of all memory waits for the CTA's output stores, for every
+//           stage (8192 x 4096 x 4096: 760 us instead of 273).
+//   read    tells that an accumulator has been read. The reads are tensor-memory ones,
+//           complete (tcgen05.wait::ld) and ordered by the tcgen05 fences on both sides;
+//           nothing else is handed over.
+__device__ __forceinline__ void arrive_landed(uint32_t addr) {
+    asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void arrive_read(uint32_t addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
                  : "memory");
 }
 // Address of the same shared-memory location in CTA `rank` of the cluster.
@@ -389,7 +414,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll 1
         for (int it = 0; it < iters; ++it, ring.next()) {
             if (!warp_wait(&landed[ring.s], ring.parity, ab, 22)) break;
-            if (lane == 0) arrive_cluster(to + ring.s * 8);
+            if (lane == 0) arrive_landed(to + ring.s * 8);
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -402,7 +427,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 for (int p = 0; p < 3 && alive; ++p, ++unit) {
                     const uint32_t idesc = instr_desc(p == 2, 256, 256);
                     const int slot = unit & 1;
-                    if (unit >= 2 && !warp_wait(&acc_empty[slot], ((unit / 2) - 1) & 1, ab, 24)) {
+                    if (unit >= 2 &&
+                        !warp_wait<CLUSTER>(&acc_empty[slot], ((unit / 2) - 1) & 1, ab, 24)) {
                         alive = false;
                         break;
                     }
@@ -410,7 +436,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     const uint32_t d = tmem + slot * 256;
 #pragma unroll 1
                     for (int k = 0; k < kblocks; ++k, ring.next()) {
-                        alive = warp_wait(&ready[ring.s], ring.parity, ab, 25);
+                        alive = warp_wait<CLUSTER>(&ready[ring.s], ring.parity, ab, 25);
                         if (!alive) break;
                         tc_fence_after();
                         const uint32_t base = smem_u32(smem + ring.s * kPairStage);
@@ -515,7 +541,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_cluster(empty0 + slot * 8);
+                if (lane == 0) arrive_read(empty0 + slot * 8);
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
