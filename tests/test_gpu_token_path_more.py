@@ -88,3 +88,35 @@ def test_the_abort_path_of_pairs_releases_its_memory_and_reports():
         got = int8_moments_matmul(x, w)
         assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
     assert device_status() == 0
+# -- beside other work on the device -----------------------------------------------------
+
+
+def test_products_in_a_row_beside_training_on_another_stream():
+    """8-bit products that are launched while the one before them ends, in both kernels,
+    while a Linear trains on another stream (its contractions hold tensor memory too):
+    every result is the one of the product alone."""
+    import triton_tagi as tt
+    from triton_tagi._lib import device_status
+    from triton_tagi.kernels import int8_moments_matmul
+
+    g = gen(40)
+    sizes = ((16, 512, 512), (40, 1000, 700), (2100, 1300, 300))
+    ops = [(operand(g, M, K), operand(g, N, K)) for M, N, K in sizes]
+    ref = [int8_moments_matmul(*o) for o in ops]
+    net = tt.Sequential([tt.Linear(256, 64, device=DEV), tt.ReLU(), tt.Linear(64, 32, device=DEV)],
+                        device=DEV)
+    x, y = randn(g, 2048, 256), randn(g, 2048, 32)
+    net.step(x, y, 0.1)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            got.append([int8_moments_matmul(*o) for o in ops])
+        with torch.cuda.stream(s2):
+            net.step(x, y, 0.1)
+    torch.cuda.synchronize()
+    assert device_status() == 0
+    for out in got:
+        for a, b in zip(out, ref):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

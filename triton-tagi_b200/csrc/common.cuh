@@ -151,6 +151,11 @@ inline unsigned grid_1d(int64_t n, int threads, int64_t max_blocks = 148 * 16) {
 // launch itself is hidden. It calls wait_for_primary() before it touches anything that
 // the one before it writes or reads; that returns when that kernel has ended and its
 // writes are visible.
+//
+// A block that waits there holds what it has taken (tensor memory, which the allocation
+// waits for when an SM has none left). So a kernel that allocates tensor memory calls
+// launch_dependents behind the allocation, once per block: no later kernel can then hold
+// columns, waiting for this one, that a block of this one still has to get.
 struct EarlyLaunch {
     dim3 grid, block;
     cudaStream_t stream;

@@ -338,7 +338,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int tiles = ctiles * ((g.M + 255) / 256);
     const int pairs = gridDim.x / 2;
     const Abort ab{&abort_flag, map_to(smem_u32(&abort_flag), rank ^ 1)};
-    launch_dependents();
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) {
@@ -361,6 +360,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                      "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        launch_dependents();  // behind the allocation: see launch_early
     }
     tc_fence_before();
     __syncthreads();
@@ -592,7 +592,6 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
     const int kblocks = (g.K + kBK - 1) / kBK;
     const int beg = share(3 * kblocks, rank, ctas), end = share(3 * kblocks, rank + 1, ctas);
     const Abort ab{&abort_flag, 0};
-    launch_dependents();
 
     // item i of this CTA's list into stage s
     auto issue = [&](int i, int s) {
@@ -625,6 +624,7 @@ __global__ void __launch_bounds__(kSplitThreads) int8_split_kernel(const Int8Arg
                      "r"(P::COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        launch_dependents();  // behind the allocation: see launch_early
     }
     tc_fence_before();
     __syncthreads();
