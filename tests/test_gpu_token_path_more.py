@@ -11,6 +11,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import test_gpu_token_path as forms
 from test_gpu_token_path import DEV, U, gen, operand, plain_linear, rand, randn, within
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +121,23 @@ def test_products_in_a_row_beside_training_on_another_stream():
     for out in got:
         for a, b in zip(out, ref):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# -- rows of every width class, and values that are not finite -----------------------------
+
+
+# 129 to 256 vectors of 4 per row: two warps per row; one vector on either side
+WIDTHS = [(5, 516), (37, 768), (3, 1020), (6, 1024), (4, 1028)]
+
+
+@pytest.mark.parametrize("R,D", WIDTHS)
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm_of_rows_of_two_warps(R, D, residual):
+    forms.test_add_rmsnorm(R, D, residual)
+    forms.test_add_rmsnorm_int8(R, D, residual)
+
+
+@pytest.mark.parametrize("R,D", WIDTHS)
+@pytest.mark.parametrize("weights", [False, True])
+def test_quantize_rows_of_two_warps(R, D, weights):
+    forms.test_quantize(R, D, weights)
