@@ -544,8 +544,8 @@ int tagi_add_rmsnorm_int8(const float* ma, const float* Sa, const float* mr, con
                           int64_t ni, float eps, void* stream);
 
 /* Rows (means m, variances S) put into 8 bits without a norm: q_m of m, q_2 of m^2
- * (weights != 0: of m^2 + S), q_S of S, scales as above. Negative variances count
- * as 0. */
+ * (weights != 0: of m^2 + S), q_S of S, scales as above. Finite negative variances
+ * count as 0. */
 int tagi_quantize_moments(const float* m, const float* S, int weights, int8_t* q_m, uint8_t* q_2,
                           uint8_t* q_S, float* scales, int64_t ldq, int64_t rows, int64_t ni,
                           void* stream);

@@ -141,3 +141,22 @@ def test_norm_of_rows_of_two_warps(R, D, residual):
 @pytest.mark.parametrize("weights", [False, True])
 def test_quantize_rows_of_two_warps(R, D, weights):
     forms.test_quantize(R, D, weights)
+
+
+@pytest.mark.parametrize("D", [5, 512, 768, 4096, 9001])
+def test_a_variance_of_minus_infinity_makes_its_row_nan(D):
+    """Not finite is not finite, on either side: codes 0 and scales NaN, where a finite
+    variance below 0 counts as 0."""
+    from triton_tagi.kernels import add_rmsnorm_int8, quantize_moments, quantize_weights
+
+    g = gen(43 + D)
+    m, S = randn(g, 5, D), rand(g, 5, D)
+    S[1, 0] = -float("inf")
+    S[2, D - 1] = -float("inf")
+    S[3, D // 2] = -1.0
+    bad = torch.tensor([False, True, True, False, False], device=DEV)
+    w, Sw = torch.ones(D, device=DEV), torch.full((D,), 0.1, device=DEV)
+    for q in (quantize_moments(m, S), quantize_weights(m.t(), S.t()),
+              add_rmsnorm_int8(m, S, None, None, w, Sw)[2]):
+        assert torch.equal(q.scales.isnan().all(0), bad) and torch.equal(q.scales.isnan().any(0), bad)
+        assert not q.q_m[bad].any() and not q.q_2[bad].any() and not q.q_S[bad].any()

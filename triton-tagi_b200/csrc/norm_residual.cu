@@ -81,9 +81,12 @@ __device__ __forceinline__ void st8(T* p, const int (&v)[VEC]) {
 
 // Magnitude of x as an ordered key: infinities and NaN above every finite value.
 __device__ __forceinline__ unsigned mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-// The same for a value that counts from 0 up: below 0 it is 0.
-__device__ __forceinline__ unsigned mag_pos(float x) { return x < 0.f ? 0u : mag(x); }
 constexpr unsigned kInfBits = 0x7f800000u;
+// The same for a value that counts from 0 up: a finite one below 0 is 0.
+__device__ __forceinline__ unsigned mag_pos(float x) {
+    const unsigned m = mag(x);
+    return x < 0.f && m < kInfBits ? 0u : m;
+}
 
 // What a row is reduced to: sum of m^2 + S, largest |p|, t and (weights) u as keys. One
 // barrier for all of them, and sums in a fixed order.

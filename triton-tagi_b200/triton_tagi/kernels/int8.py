@@ -110,7 +110,7 @@ def _quantize(m: Tensor, S: Tensor, weights: bool) -> Int8Moments:
 
 def quantize_moments(ma: Tensor, Sa: Tensor) -> Int8Moments:
     """Tokens' moments in 8 bits: the last dimension is a row; leading ones are
-    flattened. Negative variances count as 0."""
+    flattened. Finite variances below 0 count as 0."""
     return _quantize(ma, Sa, False)
 
 
