@@ -510,10 +510,11 @@ int tagi_apply_vector_sums(const double* g_m, const double* g_S, int64_t n, int 
 /* Scaled embedding lookup of n tokens: mz[t] = scale*mw[id], Sz[t] =
  * scale^2*Sw[id]. ids: n values of id_type 0 (float32, truncated toward zero,
  * V <= 2^24), 1 (int32) or 2 (int64). Ids outside [0, V) and padding_idx give
- * zero rows. mw, Sw: V x D; mz, Sz: n x D. */
+ * zero rows. mw, Sw: V x D; mz, Sz: n x D. scale and scale^2 are rounded to
+ * float32 once each. */
 int tagi_embedding_lookup(const void* ids, int id_type, const float* mw, const float* Sw,
                           float* mz, float* Sz, int64_t n, int64_t V, int64_t D,
-                          int64_t padding_idx, float scale, void* stream);
+                          int64_t padding_idx, double scale, void* stream);
 
 /* Its gradient, over tokens sorted by id: g_m[v] = scale * sum of dmz and g_S[v] =
  * scale^2 * sum of dSz over the tokens of row v (dmz, dSz: n x D). Mode
@@ -523,7 +524,7 @@ int tagi_embedding_lookup(const void* ids, int id_type, const float* mw, const f
  * leaves the others as they are. Deterministic. n <= 2^30, D <= 2^20. */
 size_t tagi_embedding_grad_workspace_size(int64_t n, int64_t D);
 int tagi_embedding_grad(const void* ids, int id_type, const float* dmz, const float* dSz,
-                        int64_t n, int64_t V, int64_t D, int64_t padding_idx, float scale,
+                        int64_t n, int64_t V, int64_t D, int64_t padding_idx, double scale,
                         int mode, float* mw, float* Sw, float* out_m, float* out_S,
                         float cap_factor, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -160,3 +160,29 @@ def test_a_variance_of_minus_infinity_makes_its_row_nan(D):
               add_rmsnorm_int8(m, S, None, None, w, Sw)[2]):
         assert torch.equal(q.scales.isnan().all(0), bad) and torch.equal(q.scales.isnan().any(0), bad)
         assert not q.q_m[bad].any() and not q.q_2[bad].any() and not q.q_S[bad].any()
+
+
+# -- scales whose squares are not exact ---------------------------------------------------
+
+
+@pytest.mark.parametrize("root", [512, 770, 3])
+def test_the_square_of_a_scale_is_rounded_once(root):
+    """scale = sqrt(512): variances scale by 512, not by the square of sqrt(512) rounded to
+    32 bits. Sums of whole numbers are exact, so results are compared for equality."""
+    from triton_tagi.kernels import embedding_grad, embedding_lookup
+
+    scale = root ** 0.5
+    g = gen(root)
+    V, D, n = 40, 24, 3000
+    ids = torch.randint(0, V, (n,), device=DEV, generator=g)
+    mw, Sw = randn(g, V, D), rand(g, V, D)
+    mz, Sz = embedding_lookup(ids, mw, Sw, scale=scale)
+    assert torch.equal(mz, mw[ids] * scale)
+    assert torch.equal(Sz, Sw[ids] * (scale * scale))
+    dm = torch.randint(-3, 4, (n, D), device=DEV, generator=g).float()
+    dS = -torch.randint(0, 4, (n, D), device=DEV, generator=g).float()
+    for k in (n, 20):  # segments that cross chunks, and ones that do not
+        t_m, t_S = (torch.zeros(V, D, device=DEV).index_add_(0, ids[:k], t[:k]) for t in (dm, dS))
+        g_m, g_S = embedding_grad(ids[:k], dm[:k], dS[:k], V, scale=scale)
+        assert torch.equal(g_m, t_m * scale)
+        assert torch.equal(g_S, t_S * (scale * scale))

@@ -609,7 +609,7 @@ using namespace tagi;
 
 extern "C" int tagi_embedding_lookup(const void* ids, int id_type, const float* mw, const float* Sw,
                                      float* mz, float* Sz, int64_t n, int64_t V, int64_t D,
-                                     int64_t padding_idx, float scale, void* stream) {
+                                     int64_t padding_idx, double scale, void* stream) {
     const char* what = "tagi_embedding_lookup";
     TAGI_REQUIRE(n >= 0 && V >= 1 && D >= 1 && V < INT32_MAX && D <= INT32_MAX, TAGI_E_BAD_ARG,
                  "%s: bad sizes", what);
@@ -619,12 +619,13 @@ extern "C" int tagi_embedding_lookup(const void* ids, int id_type, const float* 
     if (n == 0) return TAGI_OK;
     TAGI_REQUIRE(ids && mw && Sw && mz && Sz, TAGI_E_BAD_ARG, "%s: null pointer", what);
     const int vec = vec_of(D, bits_of(mw) | bits_of(Sw) | bits_of(mz) | bits_of(Sz));
-    const float s2 = scale * scale;
+    // the square is formed before either is rounded: sqrt(512) scales variances by 512
+    const float s = static_cast<float>(scale), s2 = static_cast<float>(scale * scale);
     cudaStream_t st = as_stream(stream);
 #define LOOKUP(VEC, IDT)                                                                      \
     launch_early(lookup_kernel<VEC, IDT>, {dim3(grid_1d(n * (D / VEC), 256)), dim3(256), st}, \
                  ids, mw, Sw, mz, Sz, n, static_cast<int>(V), static_cast<int>(D),            \
-                 padding_idx, scale, s2)
+                 padding_idx, s, s2)
 #define LOOKUP_V(IDT)                 \
     if (vec == 4) LOOKUP(4, IDT);     \
     else if (vec == 2) LOOKUP(2, IDT); \
@@ -641,7 +642,7 @@ extern "C" size_t tagi_embedding_grad_workspace_size(int64_t n, int64_t D) { ret
 
 extern "C" int tagi_embedding_grad(const void* ids, int id_type, const float* dmz, const float* dSz,
                                    int64_t n, int64_t V, int64_t D, int64_t padding_idx,
-                                   float scale, int mode, float* mw, float* Sw, float* out_m,
+                                   double scale, int mode, float* mw, float* Sw, float* out_m,
                                    float* out_S, float cap_factor, void* workspace,
                                    size_t workspace_bytes, void* stream) {
     const char* what = "tagi_embedding_grad";
@@ -693,8 +694,8 @@ extern "C" int tagi_embedding_grad(const void* ids, int id_type, const float* dm
     g.n = static_cast<int>(n);
     g.V = static_cast<int>(V);
     g.D = static_cast<int>(D);
-    g.s = scale;
-    g.s2 = scale * scale;
+    g.s = static_cast<float>(scale);
+    g.s2 = static_cast<float>(scale * scale);  // as in the lookup
     g.inv_cap = 1.0f / cap_factor;
     g.mw = mw;
     g.Sw = Sw;

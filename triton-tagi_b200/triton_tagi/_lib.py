@@ -68,9 +68,9 @@ _SIGS = {
     "tagi_rmsnorm_forward": "ppppppp" + "ii" + "f" + "p",
     "tagi_rmsnorm_backward": "pppppppp" + "ii" + "p",
     "tagi_apply_vector_sums": "pp" + "i" + "n" + "pppp" + "f" + "p",
-    "tagi_embedding_lookup": "pn" + "pppp" + "iiii" + "f" + "p",
+    "tagi_embedding_lookup": "pn" + "pppp" + "iiii" + "d" + "p",
     "tagi_embedding_grad_workspace_size": "ii",
-    "tagi_embedding_grad": "pn" + "pp" + "iiii" + "f" + "n" + "pppp" + "f" + "pz" + "p",
+    "tagi_embedding_grad": "pn" + "pp" + "iiii" + "d" + "n" + "pppp" + "f" + "pz" + "p",
     "tagi_add_rmsnorm_forward": "p" * 11 + "ii" + "f" + "p",
     "tagi_add_rmsnorm_int8": "p" * 12 + "iii" + "f" + "p",
     "tagi_quantize_moments": "ppn" + "pppp" + "iii" + "p",
