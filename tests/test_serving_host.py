@@ -1,0 +1,77 @@
+"""What a network from Sequential.quantize() shares with the network that it was made from,
+what it refuses and what it reports: the host side, without a GPU. Weights are laid out by
+a kernel, so where a test needs an Int8Linear it stands in empty codes for them."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import triton_tagi as tt
+from triton_tagi.layers import int8_linear
+from triton_tagi.layers.int8_linear import Int8Linear
+
+
+@pytest.fixture
+def codes(monkeypatch):
+    """Int8Linear without a GPU: codes of zeros."""
+    def zeros(mw, Sw):
+        K, N = mw.shape
+        z = torch.zeros(N, K, dtype=torch.uint8)
+        return int8_linear.Int8Moments(z.to(torch.int8), z, z, torch.zeros(3, N))
+
+    monkeypatch.setattr(int8_linear, "quantize_weights", zeros)
+
+
+def conv_net():
+    d = dict(device="cpu")
+    return tt.Sequential([tt.Conv2D(3, 4, 3, padding=1, **d), tt.ReLU(), tt.BatchNorm2D(4, **d),
+                          tt.ResBlock(4, 4, **d), tt.ResBlock(4, 8, stride=2, **d)], device="cpu")
+
+
+def every_layer(net):
+    out = []
+    for layer in net.layers:
+        out.append(layer)
+        out += [s for s in vars(layer).values() if isinstance(s, tt.Layer)]
+    return out
+
+
+# -- shared state -------------------------------------------------------------------------
+
+
+def test_a_served_network_has_layers_of_its_own():
+    """No layer, nor any inside a ResBlock, is an object of both networks; what a ResBlock
+    walks in its passes is its own too; parameters are shared."""
+    net = conv_net()
+    served = net.quantize()
+    a, b = every_layer(net), every_layer(served)
+    assert len(a) == len(b) == 5 + 6 + 9
+    assert not {id(x) for x in a} & {id(x) for x in b}
+    for block, twin in zip(net.layers[3:], served.layers[3:]):
+        own = {id(s) for s in vars(twin).values() if isinstance(s, tt.Layer)}
+        assert {id(s) for s in twin._main_layers + twin._proj_layers} == own
+        assert {id(s) for s in twin._learnable} < own
+        assert [type(s) for s in twin._main_layers] == [type(s) for s in block._main_layers]
+        assert twin.conv1.mw is block.conv1.mw and twin.bn2.Sb is block.bn2.Sb
+
+
+def test_a_served_network_starts_without_what_a_pass_left():
+    """Activations that a pass of the network keeps for its backward stay its own."""
+    net = conv_net()
+    conv, relu, bn = net.layers[:3]
+    rms = tt.RMSNorm(4, device="cpu")
+    emb = tt.Embedding(5, 4, device="cpu")
+    net.layers += [rms, emb]
+    t = torch.ones(2)
+    conv.input_ma = relu.J = bn.m_hat = rms.ma_in = rms.stream = emb._ids = t
+    net.layers[3].relu1.J = net.layers[3].conv2.delta_mw = t
+    served = net.quantize()
+    assert served.layers[0].input_ma is None and served.layers[1].J is None
+    assert served.layers[2].m_hat is None and served.layers[3].relu1.J is None
+    assert served.layers[3].conv2.delta_mw is None
+    assert served.layers[5].ma_in is None and served.layers[5].stream is None
+    assert served.layers[6]._ids is None
+    for kept in (conv.input_ma, relu.J, bn.m_hat, rms.ma_in, rms.stream, emb._ids,
+                 net.layers[3].relu1.J, net.layers[3].conv2.delta_mw):
+        assert kept is t

@@ -20,6 +20,7 @@ does with the batch sums aᵀ·δ it computes:
 
 from __future__ import annotations
 
+import copy
 from abc import ABC, abstractmethod
 
 from torch import Tensor
@@ -28,6 +29,8 @@ from torch import Tensor
 class Layer(ABC):
     """Base class for all TAGI layers."""
 
+    _kept: tuple[str, ...] = ()  # what a forward pass leaves for the backward
+
     @abstractmethod
     def forward(self, ma: Tensor, Sa: Tensor) -> tuple[Tensor, Tensor]:
         """Propagate activation means and variances forward."""
@@ -35,6 +38,15 @@ class Layer(ABC):
     @abstractmethod
     def backward(self, delta_ma: Tensor, delta_Sa: Tensor) -> tuple[Tensor, Tensor]:
         """Propagate innovation deltas backward; returns deltas for the previous layer."""
+
+    def _serving_copy(self) -> "Layer":
+        """A copy for a network that serves: the parameters are shared, but no forward
+        pass of one changes what the other keeps. (Layers that hold layers or write state
+        of their own override it.)"""
+        new = copy.copy(self)
+        for name in self._kept:
+            setattr(new, name, None)
+        return new
 
 
 class LearnableLayer(Layer):
@@ -57,6 +69,13 @@ class LearnableLayer(Layer):
     @abstractmethod
     def num_parameters(self) -> int:
         """Number of learnable scalars (means and variances)."""
+
+    def _serving_copy(self) -> "LearnableLayer":
+        new = super()._serving_copy()
+        for name in ("delta_mw", "delta_Sw", "delta_mb", "delta_Sb"):
+            if hasattr(new, name):
+                setattr(new, name, None)
+        return new
 
     # -- parameter-mode plumbing (used by Sequential) ---------------------------
     def _leaves(self) -> list["LearnableLayer"]:

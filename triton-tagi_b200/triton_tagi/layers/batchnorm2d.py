@@ -28,6 +28,8 @@ from ._params import contiguous_params
 
 
 class BatchNorm2D(LearnableLayer):
+    _kept = ("m_hat", "S_hat", "_norm_mean", "_norm_var")
+
     def __init__(self, num_features: int, momentum: float = 0.1, eps: float = 1e-5,
                  device="cuda", gain_w: float = 1.0, gain_b: float = 1.0,
                  preserve_var: bool = True) -> None:

@@ -45,6 +45,8 @@ def _channels_last(xm: Tensor, xS: Tensor) -> tuple[Tensor, Tensor]:
 
 
 class Conv2D(LearnableLayer):
+    _kept = ("input_ma",)
+
     def __init__(self, C_in: int, C_out: int, kernel_size: int, stride: int = 1,
                  padding: int = 0, padding_type: int = 1, device="cuda", init_method="He",
                  gain_w: float = 1.0, gain_b: float = 1.0, col2im_mode: str = "reference") -> None:

@@ -34,6 +34,8 @@ from ..update.parameters import update_parameters
 
 
 class Embedding(LearnableLayer):
+    _kept = ("_ids", "cat_idx")
+
     def __init__(self, num_embeddings: int, embedding_dim: int, input_size: int = 0,
                  scale: float = 1.0, padding_idx: int = -1, device="cuda",
                  out_scale: float = 1.0, sorted_grad: bool = False) -> None:

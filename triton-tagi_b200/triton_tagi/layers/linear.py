@@ -20,6 +20,8 @@ from ._params import contiguous_params, weight_apply_sums, weight_param_backward
 
 
 class Linear(LearnableLayer):
+    _kept = ("ma_in",)
+
     def __init__(self, in_features: int, out_features: int, device="cuda", init_method="He",
                  gain_w: float = 1.0, gain_b: float = 1.0, bias: bool = True) -> None:
         self.in_features = in_features

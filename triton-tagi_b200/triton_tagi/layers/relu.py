@@ -42,6 +42,8 @@ def jacobian_backward(dm: Tensor, dS: Tensor, J: Tensor) -> tuple[Tensor, Tensor
 
 
 class ReLU(Layer):
+    _kept = ("J",)
+
     def __init__(self) -> None:
         self.J = None
 

@@ -39,6 +39,8 @@ def triton_remax(mu_z: Tensor, var_z: Tensor):
 
 
 class Remax(Layer):
+    _kept = ("J",)
+
     def __init__(self) -> None:
         self.J = None
 

@@ -10,11 +10,13 @@ right/bottom padding on their first convolution (resblock.py:272-282).
 
 from __future__ import annotations
 
+import copy
+
 import torch
 from torch import Tensor
 
 from .._lib import check_cuda_f32, lib, stream
-from ..base import LearnableLayer
+from ..base import Layer, LearnableLayer
 from .batchnorm2d import BatchNorm2D
 from .conv2d import Conv2D
 from .relu import ReLU
@@ -67,20 +69,32 @@ class ResBlock(LearnableLayer):
         self.conv2 = Conv2D(out_channels, out_channels, kernel_size=3, stride=1, padding=1, **kw)
         self.relu2 = ReLU()
         self.bn2 = BatchNorm2D(out_channels, preserve_var=False, **kw)
-        self._main_layers = [self.conv1, self.relu1, self.bn1, self.conv2, self.relu2, self.bn2]
         self.use_projection = (stride != 1) or (in_channels != out_channels)
         if self.use_projection:
             self.proj_conv = Conv2D(in_channels, out_channels, kernel_size=2, stride=stride,
                                     padding=0, **kw)
             self.proj_relu = ReLU()
             self.proj_bn = BatchNorm2D(out_channels, preserve_var=False, **kw)
-            self._proj_layers = [self.proj_conv, self.proj_relu, self.proj_bn]
         else:
             self.proj_conv = self.proj_relu = self.proj_bn = None
-            self._proj_layers = []
+        self._link()
+
+    def _link(self) -> None:
+        """The two branches and the layers that learn, from the layers themselves."""
+        self._main_layers = [self.conv1, self.relu1, self.bn1, self.conv2, self.relu2, self.bn2]
+        self._proj_layers = []
         self._learnable = [self.conv1, self.bn1, self.conv2, self.bn2]
         if self.use_projection:
+            self._proj_layers = [self.proj_conv, self.proj_relu, self.proj_bn]
             self._learnable += [self.proj_conv, self.proj_bn]
+
+    def _serving_copy(self) -> "ResBlock":
+        new = copy.copy(self)
+        for name, layer in vars(self).items():
+            if isinstance(layer, Layer):
+                setattr(new, name, layer._serving_copy())
+        new._link()
+        return new
 
     def _leaves(self):
         return list(self._learnable)

@@ -27,6 +27,8 @@ from ._params import contiguous_params
 
 
 class RMSNorm(LearnableLayer):
+    _kept = ("ma_in", "inv_rms", "stream")
+
     def __init__(self, normalized_shape, eps: float = 1e-6, gain_w: float = 1.0,
                  device="cuda") -> None:
         if isinstance(normalized_shape, int):

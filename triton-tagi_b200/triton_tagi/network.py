@@ -109,11 +109,12 @@ class Sequential:
     def quantize(self) -> "Sequential":
         """A network that serves this one's predictions from 8-bit weights: its ``Linear``
         layers and attention projections as they are now, laid out once (``Int8Linear``).
-        The other layers are copies that share their parameters with this network, so
-        quantize again after training on. Only ``forward`` works on it."""
+        The other layers are copies that share their parameters with this network, and
+        nothing else: passes of the two do not disturb one another. Quantize again after
+        training on. Only ``forward`` works on it."""
         net = copy.copy(self)
         net.layers = [layer.quantize() if isinstance(layer, (Linear, MultiheadAttentionV2))
-                      else copy.copy(layer) for layer in self.layers]
+                      else layer._serving_copy() for layer in self.layers]
         net.serving, net.reducer, net._graph = True, None, None
         return net
 
