@@ -1,0 +1,104 @@
+"""Serving and training side by side on a GPU: what a network from Sequential.quantize()
+leaves alone, what it answers and what it reports."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_token_path import DEV, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def conv_net(seed=0):
+    import triton_tagi as tt
+
+    torch.manual_seed(seed)
+    d = dict(device=DEV, gain_w=0.3, gain_b=0.3)
+    return tt.Sequential([tt.Conv2D(3, 8, 3, padding=1, **d), tt.ReLU(), tt.BatchNorm2D(8, **d),
+                          tt.ResBlock(8, 8, **d), tt.ResBlock(8, 16, stride=2, **d),
+                          tt.AvgPool2D(2), tt.Flatten(), tt.Linear(16 * 4 * 4, 10, device=DEV)],
+                         device=DEV)
+
+
+def conv_batch(n, seed):
+    g = gen(seed)
+    return randn(g, n, 3, 16, 16), randn(g, n, 10)
+
+
+def everything(net):
+    """Parameters and running statistics, in network order."""
+    return [getattr(leaf, n) for leaf in net.leaves()
+            for n in ("mw", "Sw", "mb", "Sb", "running_mean", "running_var")
+            if getattr(leaf, n, None) is not None]
+
+
+def test_serving_between_the_passes_of_a_network_disturbs_nothing():
+    """Forward, a served batch of another size, backward: the deltas and the updates are
+    those of a network that nobody served from."""
+    from triton_tagi._chain import backward_chain
+
+    x, _ = conv_batch(12, 1)
+    other, _ = conv_batch(5, 2)
+    g = gen(3)
+    dm, dS = randn(g, 12, 10) * 0.1, -randn(g, 12, 10).abs() * 0.1
+    out = []
+    for serve in (False, True):
+        net = conv_net()
+        served = net.quantize()
+        net.forward(x)
+        if serve:
+            served.forward(other)
+        deltas = backward_chain(net.layers, dm, dS)
+        for layer in net.learnable_layers():
+            layer.update(2.0)
+        out.append([*deltas, *(t for leaf in net.leaves() for t in (leaf.mw, leaf.Sw))])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
+def test_a_network_trains_on_as_if_nobody_had_served_from_it():
+    """Served batches between steps, before and after the first one (which initialises the
+    BatchNorms): parameters, running statistics and flags are those of a network apart."""
+    out = []
+    for serve in (False, True):
+        net = conv_net()
+        served = net.quantize()
+        for k in range(3):
+            if serve:
+                served.forward(conv_batch(5, 10 + k)[0])
+                served.eval()
+            net.step(*conv_batch(12, k), 0.1)
+            served = net.quantize()
+        assert all(f for f in net._modes() if f is not None)
+        out.append([t.clone() for t in everything(net)])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
+def test_a_served_convolution_network_predicts_as_its_eval_mode_does():
+    """The Linear head in 8 bits behind the network's own eval pass; a later step of the
+    network moves its running statistics and not the served ones."""
+    net = conv_net()
+    for k in range(3):
+        net.step(*conv_batch(12, k), 0.1)
+    served = net.quantize()
+    x, _ = conv_batch(6, 20)
+    mu, var = served.forward(x)
+    net.eval()
+    h = net.layers[0].forward(x, torch.zeros_like(x))
+    for layer in net.layers[1:-1]:
+        h = layer.forward(*h)
+    ref_mu, ref_var = net.layers[-1].quantize().forward(*h)
+    assert torch.equal(mu, ref_mu) and torch.equal(var, ref_var)
+    net.train()
+    stats = [t.clone() for leaf in net.leaves() if hasattr(leaf, "running_mean")
+             for t in (leaf.running_mean, leaf.running_var)]
+    net.step(*conv_batch(12, 3), 0.1)
+    now = [t for leaf in net.leaves() if hasattr(leaf, "running_mean")
+           for t in (leaf.running_mean, leaf.running_var)]
+    assert not any(torch.equal(a, b) for a, b in zip(stats, now))
+    own = [t for leaf in served.leaves() if hasattr(leaf, "running_mean")
+           for t in (leaf.running_mean, leaf.running_var)]
+    assert len(own) == len(stats) and all(torch.equal(a, b) for a, b in zip(stats, own))

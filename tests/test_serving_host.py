@@ -75,3 +75,29 @@ def test_a_served_network_starts_without_what_a_pass_left():
     for kept in (conv.input_ma, relu.J, bn.m_hat, rms.ma_in, rms.stream, emb._ids,
                  net.layers[3].relu1.J, net.layers[3].conv2.delta_mw):
         assert kept is t
+
+
+def test_a_served_network_is_in_eval_mode_with_statistics_of_its_own():
+    net = conv_net()
+    flags = net._modes()
+    for bn in (net.layers[2], net.layers[4].proj_bn):
+        bn._stats_allreduce, bn._stats_world = (lambda sums: None), 4
+    served = net.quantize()
+    served.eval()
+    assert net._modes() == flags and all(f for f in flags if f is not None)
+    norms = [(a, b) for a, b in zip(every_layer(net), every_layer(served))
+             if isinstance(a, tt.BatchNorm2D)]
+    assert len(norms) == 6
+    for a, b in norms:
+        assert a.training and not b.training
+        assert b._stats_allreduce is None and b._stats_world == 1
+        assert torch.equal(a.running_mean, b.running_mean)
+        assert a.running_mean.data_ptr() != b.running_mean.data_ptr()
+        assert a.running_var.data_ptr() != b.running_var.data_ptr()
+    assert net.layers[2]._stats_allreduce is not None
+    assert not any(block.training for block in served.layers[3:])
+    with pytest.raises(RuntimeError, match="serves forward"):
+        served.train()
+    assert not served.layers[2].training
+    net.train()
+    assert net.layers[2].training and not served.layers[2].training

@@ -55,6 +55,13 @@ class BatchNorm2D(LearnableLayer):
         self._stats_allreduce = None
         self._stats_world = 1
 
+    def _serving_copy(self) -> "BatchNorm2D":
+        new = super()._serving_copy()
+        new.running_mean = self.running_mean.clone()
+        new.running_var = self.running_var.clone()
+        new._stats_allreduce, new._stats_world = None, 1  # one process serves alone
+        return new
+
     def train(self) -> None:
         self.training = True
 

@@ -110,18 +110,23 @@ class Sequential:
         """A network that serves this one's predictions from 8-bit weights: its ``Linear``
         layers and attention projections as they are now, laid out once (``Int8Linear``).
         The other layers are copies that share their parameters with this network, and
-        nothing else: passes of the two do not disturb one another. Quantize again after
-        training on. Only ``forward`` works on it."""
+        nothing else: passes of the two do not disturb one another. They are in eval mode:
+        a BatchNorm2D serves with a copy of its running statistics as they are now.
+        Quantize again after training on. Only ``forward`` works on it."""
         net = copy.copy(self)
         net.layers = [layer.quantize() if isinstance(layer, (Linear, MultiheadAttentionV2))
                       else layer._serving_copy() for layer in self.layers]
         net.serving, net.reducer, net._graph = True, None, None
+        net.eval()
         return net
 
-    def step(self, x_batch: Tensor, y_batch: Tensor, sigma_v: float) -> tuple[Tensor, Tensor]:
+    def _refuse_serving(self) -> None:
         if self.serving:
             raise RuntimeError("a quantized network serves forward passes only; train the "
                                "network that it was made from")
+
+    def step(self, x_batch: Tensor, y_batch: Tensor, sigma_v: float) -> tuple[Tensor, Tensor]:
+        self._refuse_serving()
         red = self.reducer
         if self.cuda_graph and x_batch.is_cuda and (
                 red is None or getattr(red, "capturable", False)):
@@ -202,6 +207,7 @@ class Sequential:
         self._graph = None
 
     def train(self) -> None:
+        self._refuse_serving()
         for layer in self.layers:
             if hasattr(layer, "training"):
                 layer.train()
