@@ -101,3 +101,27 @@ def test_a_served_network_is_in_eval_mode_with_statistics_of_its_own():
     assert not served.layers[2].training
     net.train()
     assert net.layers[2].training and not served.layers[2].training
+
+
+# -- a served network as a Sequential -----------------------------------------------------
+
+
+def token_net(E=8, V=12):
+    d = dict(device="cpu")
+    return tt.Sequential([tt.Embedding(V, E, **d), tt.MultiheadAttentionV2(E, 2, 6, bias=True, **d),
+                          tt.RMSNorm(E, **d), tt.Linear(E, V, **d)], device="cpu")
+
+
+def test_a_served_network_counts_its_parameters(codes):
+    net = token_net()
+    served = net.quantize()
+    assert isinstance(served.layers[1].k_proj, Int8Linear)
+    assert served.layers[3].num_parameters == net.layers[3].num_parameters
+    assert served.layers[1].num_parameters == net.layers[1].num_parameters
+    assert served.num_parameters() == net.num_parameters()
+    # what learns: the layers that own parameters in 32 bits
+    assert [type(x) for x in served.leaves()] == [tt.Embedding, tt.RMSNorm]
+    assert len(net.leaves()) == 6
+    for call in (served.layers[1].update, served.layers[3].update):
+        with pytest.raises(RuntimeError, match="serves a trained layer"):
+            call(2.0)

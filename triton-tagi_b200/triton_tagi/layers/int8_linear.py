@@ -49,5 +49,13 @@ class Int8Linear(Layer):
     def backward(self, delta_ma: Tensor, delta_Sa: Tensor) -> tuple[Tensor, Tensor]:
         raise RuntimeError("Int8Linear serves a trained layer: it has no backward pass")
 
+    def update(self, cap_factor: float) -> None:
+        raise RuntimeError("Int8Linear serves a trained layer: it has no update")
+
+    @property
+    def num_parameters(self) -> int:
+        """As the ``Linear``'s: means and variances of weights and biases."""
+        return 2 * (self.in_features + (1 if self.has_bias else 0)) * self.out_features
+
     def __repr__(self) -> str:
         return f"Int8Linear(in={self.in_features}, out={self.out_features}, bias={self.has_bias})"

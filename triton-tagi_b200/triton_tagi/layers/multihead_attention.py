@@ -57,7 +57,8 @@ class MultiheadAttentionV2(LearnableLayer):
         self._attn_mu = self._attn_var = None
 
     def _leaves(self):
-        return [self.q_proj, self.k_proj, self.v_proj]
+        return [p for p in (self.q_proj, self.k_proj, self.v_proj)
+                if isinstance(p, LearnableLayer)]  # none in 8 bits
 
     def forward(self, ma: Tensor, Sa: Tensor) -> tuple[Tensor, Tensor]:
         B, S, E = ma.shape

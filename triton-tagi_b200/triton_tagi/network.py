@@ -48,6 +48,7 @@ from torch import Tensor
 from ._chain import backward_chain, forward_chain
 from ._lib import check_device_status
 from .base import LearnableLayer
+from .layers.int8_linear import Int8Linear
 from .layers.linear import Linear
 from .layers.multihead_attention import MultiheadAttentionV2
 from .layers.resblock import ResBlock
@@ -224,7 +225,8 @@ class Sequential:
         return "\n".join(lines + [")"])
 
     def num_parameters(self) -> int:
-        return sum(layer.num_parameters for layer in self.learnable_layers())
+        return sum(layer.num_parameters for layer in self.layers
+                   if isinstance(layer, (LearnableLayer, Int8Linear)))
 
     def get_attention_scores(self) -> dict[int, tuple[Tensor, Tensor]]:
         out = {i: layer.get_attention_scores() for i, layer in enumerate(self.layers)
