@@ -125,3 +125,30 @@ def test_a_served_network_counts_its_parameters(codes):
     for call in (served.layers[1].update, served.layers[3].update):
         with pytest.raises(RuntimeError, match="serves a trained layer"):
             call(2.0)
+
+
+def test_checkpoints_of_a_served_network_are_refused(codes, tmp_path):
+    """A file would lack the 8-bit layers; loading one would write the parameters that the
+    served network shares, beside 8-bit weights of before."""
+    from triton_tagi.checkpoint import net_state, restore_net_state
+
+    net = token_net()
+    served = net.quantize()
+    run = tt.RunDir("d", "a", "o", base=str(tmp_path))
+    path = run.save_checkpoint(net, 1, {})
+    before = [t.clone() for leaf in net.leaves() for t in (leaf.mw, leaf.Sw)]
+    for leaf in net.leaves():
+        leaf.mw.add_(1.0)
+    moved = [t.clone() for leaf in net.leaves() for t in (leaf.mw, leaf.Sw)]
+    mixed = tt.Sequential([served.layers[3]], device="cpu")  # built by hand
+    for call in (lambda: run.save_checkpoint(served, 2, {}), lambda: net_state(served),
+                 lambda: net_state(mixed), lambda: restore_net_state(mixed, {}),
+                 lambda: run.load_checkpoint(served, path),
+                 lambda: tt.load_model(path, lambda cfg: served, device="cpu")):
+        with pytest.raises(RuntimeError, match="8 bits"):
+            call()
+    assert [p.name for p in run.checkpoints.iterdir()] == [path.name]
+    now = [t for leaf in net.leaves() for t in (leaf.mw, leaf.Sw)]
+    assert all(torch.equal(a, b) for a, b in zip(now, moved))
+    run.load_checkpoint(net, path)  # the network itself
+    assert torch.equal(net.layers[0].mw, before[0])

@@ -15,6 +15,8 @@ where ``attr`` runs over ``mw, Sw, mb, Sb, running_mean, running_var`` (those
 the layer has) and containers with sub-layers (``ResBlock``) store a list in
 their ``_learnable`` order (conv1, bn1, conv2, bn2[, proj_conv, proj_bn]).
 Loading copies into the existing parameter tensors, on the network's device.
+Networks that hold layers in 8 bits (``Sequential.quantize()``) are neither saved nor
+loaded: the file has no place for codes. Save the network itself and quantize it again.
 """
 
 from __future__ import annotations
@@ -28,6 +30,7 @@ from typing import Any, Callable
 import torch
 
 from .base import LearnableLayer
+from .layers.int8_linear import Int8Linear
 from .network import Sequential
 
 STATE_ATTRS = ("mw", "Sw", "mb", "Sb", "running_mean", "running_var")
@@ -39,8 +42,15 @@ def layer_state(layer) -> dict[str, torch.Tensor]:
             if getattr(layer, a, None) is not None}
 
 
+def _refuse_codes(net: Sequential) -> None:
+    if getattr(net, "serving", False) or any(isinstance(x, Int8Linear) for x in net.layers):
+        raise RuntimeError("a checkpoint cannot hold layers in 8 bits: save or load the network "
+                           "that this one was made from, and quantize it again")
+
+
 def net_state(net: Sequential) -> dict[int, Any]:
     """``net_state`` of a checkpoint: learnable layers by their index."""
+    _refuse_codes(net)
     out: dict[int, Any] = {}
     for i, layer in enumerate(net.layers):
         subs = getattr(layer, "_learnable", None)
@@ -63,6 +73,7 @@ def _copy_into(layer, saved: dict[str, torch.Tensor], device: torch.device) -> N
 
 def restore_net_state(net: Sequential, state: dict[int, Any]) -> None:
     """Copy a checkpoint's ``net_state`` into ``net``'s parameter tensors."""
+    _refuse_codes(net)
     for i, layer in enumerate(net.layers):
         saved = state.get(i)
         if saved is None:
