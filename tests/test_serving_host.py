@@ -152,3 +152,29 @@ def test_checkpoints_of_a_served_network_are_refused(codes, tmp_path):
     assert all(torch.equal(a, b) for a, b in zip(now, moved))
     run.load_checkpoint(net, path)  # the network itself
     assert torch.equal(net.layers[0].mw, before[0])
+
+
+def test_a_linear_too_long_for_8_bits_stays_in_32(codes):
+    """More than 33025 inputs: the layer alone refuses, a network serves it in 32 bits."""
+    long = tt.Linear(Int8Linear.MAX_IN + 1, 2, device="cpu")
+    long.ma_in = torch.ones(1)
+    net = tt.Sequential([long, tt.Linear(2, 3, device="cpu"),
+                         tt.Linear(Int8Linear.MAX_IN, 1, device="cpu")], device="cpu")
+    with pytest.raises(ValueError, match="33025"):
+        long.quantize()
+    served = net.quantize()
+    assert [type(x) for x in served.layers] == [tt.Linear, Int8Linear, Int8Linear]
+    assert served.layers[0] is not long and served.layers[0].mw is long.mw
+    assert served.layers[0].ma_in is None and long.ma_in is not None
+    assert served.num_parameters() == net.num_parameters()
+
+
+def test_an_attention_too_wide_for_8_bits_stays_in_32(codes, monkeypatch):
+    monkeypatch.setattr(Int8Linear, "MAX_IN", 7)
+    net = token_net()  # projections of 8 inputs
+    served = net.quantize()
+    mha, own = served.layers[1], net.layers[1]
+    for a, b in zip((mha.q_proj, mha.k_proj, mha.v_proj), (own.q_proj, own.k_proj, own.v_proj)):
+        assert type(a) is tt.Linear and a is not b and a.mw is b.mw
+    with pytest.raises(RuntimeError, match="serves forward"):
+        served.step(None, None, 0.1)

@@ -81,6 +81,13 @@ class Linear(LearnableLayer):
 
         return Int8Linear(self)
 
+    def _serving(self):
+        """For a network that serves: in 8 bits, or a copy where the reduction is too long
+        for them."""
+        from .int8_linear import Int8Linear
+
+        return self.quantize() if self.in_features <= Int8Linear.MAX_IN else self._serving_copy()
+
     def update(self, cap_factor: float) -> None:
         weight_update(self, cap_factor, self.has_bias)
 

@@ -104,11 +104,11 @@ class MultiheadAttentionV2(LearnableLayer):
         return a[0] + b[0] + v[0], a[1] + b[1] + v[1]
 
     def quantize(self) -> "MultiheadAttentionV2":
-        """This layer as it is now for serving: its projections in 8 bits (inference
-        only)."""
+        """This layer as it is now for serving: its projections in 8 bits (inference only;
+        copies in 32 bits where ``embed_dim`` is too long for them)."""
         new = copy.copy(self)
         new.q_proj, new.k_proj, new.v_proj = (
-            p.quantize() if isinstance(p, Linear) else p
+            p._serving() if isinstance(p, Linear) else p
             for p in (self.q_proj, self.k_proj, self.v_proj))
         new._cache = new._attn_mu = new._attn_var = None
         return new

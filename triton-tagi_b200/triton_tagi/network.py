@@ -109,13 +109,15 @@ class Sequential:
 
     def quantize(self) -> "Sequential":
         """A network that serves this one's predictions from 8-bit weights: its ``Linear``
-        layers and attention projections as they are now, laid out once (``Int8Linear``).
+        layers and attention projections as they are now, laid out once (``Int8Linear``;
+        those of more inputs than that takes stay in 32 bits).
         The other layers are copies that share their parameters with this network, and
         nothing else: passes of the two do not disturb one another. They are in eval mode:
         a BatchNorm2D serves with a copy of its running statistics as they are now.
         Quantize again after training on. Only ``forward`` works on it."""
         net = copy.copy(self)
-        net.layers = [layer.quantize() if isinstance(layer, (Linear, MultiheadAttentionV2))
+        net.layers = [layer._serving() if isinstance(layer, Linear)
+                      else layer.quantize() if isinstance(layer, MultiheadAttentionV2)
                       else layer._serving_copy() for layer in self.layers]
         net.serving, net.reducer, net._graph = True, None, None
         net.eval()
