@@ -102,3 +102,42 @@ def test_a_served_convolution_network_predicts_as_its_eval_mode_does():
     own = [t for leaf in served.leaves() if hasattr(leaf, "running_mean")
            for t in (leaf.running_mean, leaf.running_var)]
     assert len(own) == len(stats) and all(torch.equal(a, b) for a, b in zip(stats, own))
+
+
+def token_net(check_device=None, V=48, E=64, S=12):
+    import triton_tagi as tt
+
+    torch.manual_seed(1)
+    d = dict(device=DEV)
+    return tt.Sequential([tt.Embedding(V, E, scale=0.25, **d), tt.MultiheadAttentionV2(E, 4, S, **d),
+                          tt.RMSNorm(E, **d), tt.Linear(E, V, **d)], device=DEV,
+                         check_device=check_device)
+
+
+def tokens(V=48, S=12, B=8):
+    return torch.randint(0, V, (B, S), device=DEV, generator=gen(5)).float()
+
+
+def test_a_served_forward_whose_kernel_gave_up_raises():
+    """The host's limit makes the 8-bit kernels give up; with check_device the forward pass
+    says so, and the next one is as before. A captured pass is not read (nothing has run)."""
+    from triton_tagi._lib import device_status, set_wait_limit_ns
+
+    served = token_net(check_device=True).quantize()
+    x = tokens()
+    ref = served.forward(x)
+    set_wait_limit_ns(500)
+    try:
+        with pytest.raises(RuntimeError, match="gave up"):
+            served.forward(x)
+    finally:
+        set_wait_limit_ns(0)
+    assert device_status() == 0
+    got = served.forward(x)
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = served.forward(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])

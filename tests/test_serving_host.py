@@ -178,3 +178,19 @@ def test_an_attention_too_wide_for_8_bits_stays_in_32(codes, monkeypatch):
         assert type(a) is tt.Linear and a is not b and a.mw is b.mw
     with pytest.raises(RuntimeError, match="serves forward"):
         served.step(None, None, 0.1)
+
+
+@pytest.mark.parametrize("check", [True, False])
+def test_a_served_forward_reads_the_error_word(monkeypatch, check):
+    """check_device covers what a served network does, its forward passes: without it a
+    kernel that gave up would leave unwritten predictions and no word."""
+    from triton_tagi import network
+
+    read = []
+    monkeypatch.setattr(network, "check_device_status", lambda: read.append(1))
+    net = tt.Sequential([tt.Flatten()], device="cpu", check_device=check)
+    x = torch.zeros(2, 3, 4)
+    net.forward(x)
+    assert not read  # step() reads it for a network that trains
+    net.quantize().forward(x)
+    assert len(read) == (1 if check else 0)

@@ -29,9 +29,10 @@ captured graph is keyed on the input shapes, σ_v, ``fuse_update`` and every
 layer's training flag, so ``train()`` / ``eval()`` lead to a new capture.
 
 ``check_device=True`` (or the environment variable ``TAGI_B200_CHECK=1``) reads
-the tensor-core kernels' error word after every step (this synchronises) and
-raises ``RuntimeError`` if a bounded wait inside a kernel ran out, in which case
-that kernel's outputs are incomplete.
+the tensor-core kernels' error word after every step, or on a served network after
+every forward pass that is not being captured (this synchronises), and raises
+``RuntimeError`` if a bounded wait inside a kernel ran out, in which case that kernel's
+outputs are incomplete.
 
 ``quantize()`` gives a network for serving: the same layers with every ``Linear`` (and
 the projections of attention layers) in 8 bits, for ``forward`` only.
@@ -105,7 +106,11 @@ class Sequential:
         return out
 
     def forward(self, x: Tensor) -> tuple[Tensor, Tensor]:
-        return forward_chain(self.layers, x, torch.zeros_like(x))
+        out = forward_chain(self.layers, x, torch.zeros_like(x))
+        if (self.serving and self.check_device
+                and not (x.is_cuda and torch.cuda.is_current_stream_capturing())):
+            check_device_status()
+        return out
 
     def quantize(self) -> "Sequential":
         """A network that serves this one's predictions from 8-bit weights: its ``Linear``
