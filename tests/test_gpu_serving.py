@@ -141,3 +141,58 @@ def test_a_served_forward_whose_kernel_gave_up_raises():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+
+
+@pytest.mark.parametrize("mode", ["deltas", "update"])
+def test_rmsnorm_of_several_rows_per_token(mode):
+    """RMSNorm(32) on tokens of 96 norms three rows each: with a residual, and in the
+    backward pass, it gives what the same rows give apart."""
+    import triton_tagi as tt
+
+    g = gen(7)
+    shape = (4, 5, 96)
+    ma, mr, dm, xm = (randn(g, *shape) for _ in range(4))
+    Sa, Sr, dS, xS = (randn(g, *shape).abs() * 0.1 for _ in range(4))
+    a, b = tt.RMSNorm(32, device=DEV), tt.RMSNorm(32, device=DEV)
+    rows = lambda t: t.view(-1, 32)  # noqa: E731
+    for layer in (a, b):
+        layer._set_param_mode(mode, 2.0)
+    got = a.forward(ma, Sa, residual=(mr, Sr))
+    ref = b.forward(rows(ma), rows(Sa), residual=(rows(mr), rows(Sr)))
+    for x, y in zip((*got, *a.stream), (*ref, *b.stream)):
+        assert x.shape == shape and torch.equal(rows(x), y)
+    got = a.backward(dm, dS, stream_delta=(xm, xS))
+    ref = b.backward(rows(dm), rows(dS), stream_delta=(rows(xm), rows(xS)))
+    for x, y in zip(got, ref):
+        assert x.shape == shape and torch.equal(rows(x), y)
+    if mode == "deltas":
+        assert torch.equal(a.delta_mw, b.delta_mw) and torch.equal(a.delta_Sw, b.delta_Sw)
+    assert torch.equal(a.mw, b.mw) and torch.equal(a.Sw, b.Sw)
+    q, p = a.forward_int8(ma, Sa, residual=(mr, Sr)), b.forward_int8(rows(ma), rows(Sa),
+                                                                     residual=(rows(mr), rows(Sr)))
+    assert all(torch.equal(x, y) for x, y in zip(q, p))
+    assert a.stream[0].shape == shape and torch.equal(rows(a.stream[1]), b.stream[1])
+    with pytest.raises(ValueError, match="rows of 32"):
+        a.forward(ma[..., :50].contiguous(), Sa[..., :50].contiguous(),
+                  residual=(mr[..., :50], Sr[..., :50]))
+    with pytest.raises(ValueError, match="shape"):  # as many values, other rows
+        a.forward(ma, Sa, residual=(mr.view(5, 4, 96), Sr.view(5, 4, 96)))
+
+
+def test_a_norm_of_several_rows_per_token_is_served():
+    """In front of an Int8Linear of the whole token the norm's codes would be rows of
+    another width: the served network norms in 32 bits there."""
+    import triton_tagi as tt
+
+    torch.manual_seed(2)
+    net = tt.Sequential([tt.Linear(16, 96, device=DEV), tt.RMSNorm(32, device=DEV),
+                         tt.Linear(96, 10, device=DEV)], device=DEV)
+    x = randn(gen(8), 6, 16)
+    mu, var = net.forward(x)
+    served = net.quantize()
+    q_mu, q_var = served.forward(x)
+    h = served.layers[1].forward(*served.layers[0].forward(x, torch.zeros_like(x)))
+    ref = served.layers[2].forward(*h)
+    assert torch.equal(q_mu, ref[0]) and torch.equal(q_var, ref[1])
+    rms = lambda t: t.double().square().mean().sqrt().item()  # noqa: E731
+    assert rms(q_mu - mu) <= 0.05 * rms(mu) and rms(q_var - var) <= 0.1 * rms(var)

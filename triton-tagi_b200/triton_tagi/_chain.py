@@ -7,7 +7,7 @@ container may apply between neighbours (the results are the layers' own):
   takes its bias sums (the per-channel sums of its output deltas) from the
   BatchNorm's backward launch instead of a pass of its own;
 * an RMSNorm directly before an Int8Linear (a network that serves) writes that
-  layer's 8-bit operand itself.
+  layer's 8-bit operand itself, where a token is one of its rows.
 
 Forward fusions of the ReLU were measured and dropped: applied in the epilogue
 of the contraction before it, the exp/erf of the rectified moments at the end of
@@ -40,7 +40,7 @@ def forward_chain(layers, ma: Tensor, Sa: Tensor) -> tuple[Tensor, Tensor]:
             ma, Sa = layer.forward_int8(codes, ma.shape[:-1])
             codes = None
         elif (isinstance(layer, RMSNorm) and i + 1 < len(layers)
-                and isinstance(layers[i + 1], Int8Linear)):
+                and isinstance(layers[i + 1], Int8Linear) and ma.shape[-1] == layer.ni):
             codes = layer.forward_int8(ma, Sa)
         else:
             ma, Sa = layer.forward(ma, Sa)

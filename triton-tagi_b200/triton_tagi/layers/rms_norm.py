@@ -51,6 +51,20 @@ class RMSNorm(LearnableLayer):
         self._input_shape = None
         self.delta_mw = self.delta_Sw = self.delta_mb = self.delta_Sb = None
 
+    def _rows_of(self, *ts: Tensor | None) -> tuple:
+        """The tensors, of one shape, with rows of ``ni``: as they are, or split where the
+        last dimension is a multiple of it (what does not fit, the kernels refuse)."""
+        shape = ts[0].shape
+        if not shape or shape[-1] == self.ni or shape[-1] % self.ni:
+            return ts
+        if any(t is not None and t.shape != shape for t in ts):
+            raise ValueError(f"RMSNorm: a shape differs from {tuple(shape)}")
+        return tuple(None if t is None else t.reshape(-1, self.ni) for t in ts)
+
+    @staticmethod
+    def _shaped(shape: torch.Size, *ts: Tensor) -> tuple:
+        return ts if ts[0].shape == shape else tuple(t.view(shape) for t in ts)
+
     def forward(self, ma: Tensor, Sa: Tensor,
                 residual: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
         check_cuda_f32(ma, Sa)
@@ -58,9 +72,11 @@ class RMSNorm(LearnableLayer):
         self._input_shape = ma.shape
         self.stream = None
         if residual is not None:
-            hm, hS, mz, Sz, inv = add_rmsnorm(ma, Sa, *residual, self.mw, self.Sw, float(self.eps))
-            self.stream = (hm, hS)
+            hm, hS, mz, Sz, inv = add_rmsnorm(*self._rows_of(ma, Sa, *residual), self.mw, self.Sw,
+                                              float(self.eps))
             self.ma_in, self.inv_rms = hm.view(-1, self.ni), inv.view(-1, 1)
+            hm, hS, mz, Sz = self._shaped(ma.shape, hm, hS, mz, Sz)
+            self.stream = (hm, hS)
             return mz, Sz
         a = ma.reshape(-1, self.ni).contiguous()
         s = Sa.reshape(-1, self.ni).contiguous()
@@ -76,19 +92,20 @@ class RMSNorm(LearnableLayer):
 
     def forward_int8(self, ma: Tensor, Sa: Tensor,
                      residual: tuple[Tensor, Tensor] | None = None) -> Int8Moments:
-        """The output in 8 bits, leading dimensions flattened to rows (inference only:
+        """The output in 8 bits, flattened to rows of ``normalized_shape`` (inference only:
         nothing is kept for a backward but ``stream``)."""
         contiguous_params(self, ("mw", "Sw"))
         mr, Sr = (None, None) if residual is None else residual
-        hm, hS, q = add_rmsnorm_int8(ma, Sa, mr, Sr, self.mw, self.Sw, float(self.eps))
-        self.stream = None if residual is None else (hm, hS)
+        hm, hS, q = add_rmsnorm_int8(*self._rows_of(ma, Sa, mr, Sr), self.mw, self.Sw,
+                                     float(self.eps))
+        self.stream = None if residual is None else self._shaped(ma.shape, hm, hS)
         self.ma_in = self.inv_rms = None
         return q
 
     def _fused_backward(self, dmz, dSz, delta) -> tuple[Tensor, Tensor]:
-        mode = self._param_mode
+        mode, shape = self._param_mode, dmz.shape
+        dmz, dSz, rm, rS = self._rows_of(dmz, dSz, *((None, None) if delta is None else delta))
         head = (dmz, dSz, self.ma_in, self.inv_rms)
-        rm, rS = (None, None) if delta is None else delta
         if mode == "deltas":
             d_m, d_S, self.delta_mw, self.delta_Sw = add_rmsnorm_backward(
                 *head, self.mw, self.Sw, rm, rS)
@@ -101,7 +118,7 @@ class RMSNorm(LearnableLayer):
             self._reducer.ready(self)
         else:
             raise ValueError(f"unknown parameter mode {mode!r}")
-        return d_m, d_S
+        return self._shaped(shape, d_m, d_S)
 
     def backward(self, delta_mz: Tensor, delta_Sz: Tensor,
                  stream_delta: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
