@@ -196,3 +196,47 @@ def test_a_norm_of_several_rows_per_token_is_served():
     assert torch.equal(q_mu, ref[0]) and torch.equal(q_var, ref[1])
     rms = lambda t: t.double().square().mean().sqrt().item()  # noqa: E731
     assert rms(q_mu - mu) <= 0.05 * rms(mu) and rms(q_var - var) <= 0.1 * rms(var)
+
+
+def test_a_stream_changed_in_place_is_refused_by_the_backward():
+    """The stream is what the backward pass reads: an addition into it, by this library or
+    by torch, would silently change gamma's deltas. A sum of its own is the way."""
+    import triton_tagi as tt
+    from triton_tagi.layers.resblock import triton_add_shortcut
+
+    g = gen(9)
+    ma, mr, dm, xm = (randn(g, 6, 64) for _ in range(4))
+    Sa, Sr, dS, xS = (randn(g, 6, 64).abs() * 0.1 for _ in range(4))
+    norm = tt.RMSNorm(64, device=DEV)
+    norm.forward(ma, Sa, residual=(mr, Sr))
+    hm, hS = norm.stream
+    kept = hm.clone(), hS.clone()
+    out = tt.Add().forward(*norm.stream, xm, xS)
+    assert torch.equal(out[0], hm + xm) and torch.equal(hm, kept[0]) and torch.equal(hS, kept[1])
+    ref = norm.backward(dm, dS, stream_delta=(xm, xS))
+    d_w = norm.delta_mw
+    for change in (lambda: triton_add_shortcut(xm, xS, hm, hS), lambda: hm.add_(xm),
+                   lambda: hm.view(-1)[:3].zero_()):
+        norm.forward(ma, Sa, residual=(mr, Sr))
+        hm, hS = norm.stream
+        change()
+        with pytest.raises(RuntimeError, match="changed in place"):
+            norm.backward(dm, dS, stream_delta=(xm, xS))
+    norm.forward(ma, Sa, residual=(mr, Sr))
+    got = norm.backward(dm, dS, stream_delta=(xm, xS))
+    assert all(torch.equal(a, b) for a, b in zip(got, ref)) and torch.equal(norm.delta_mw, d_w)
+
+
+def test_a_residual_pass_in_inference_mode():
+    """Tensors that count no changes are not asked for them."""
+    import triton_tagi as tt
+    from triton_tagi.layers.resblock import triton_add_shortcut
+
+    g = gen(10)
+    norm = tt.RMSNorm(64, device=DEV)
+    with torch.inference_mode():
+        a, b = randn(g, 4, 64), randn(g, 4, 64).abs()
+        norm.forward(a, b, residual=(a, b))
+        d_m, _ = norm.backward(a, b)
+        triton_add_shortcut(a, b, *norm.stream)
+    assert torch.isfinite(d_m).all()

@@ -32,6 +32,9 @@ def triton_add_shortcut(mu_s: Tensor, var_s: Tensor, mu_a: Tensor, var_a: Tensor
     mu_s, var_s = mu_s.contiguous(), var_s.contiguous()
     lib()("tagi_add_inplace", mu_a.data_ptr(), var_a.data_ptr(), mu_s.data_ptr(),
           var_s.data_ptr(), mu_a.numel(), stream(mu_a))
+    # torch counts changes in place (but for inference tensors); a layer may have kept these
+    torch.autograd.graph.increment_version(
+        [t for t in (mu_a, var_a) if not t.is_inference()])
 
 
 triton_delta_merge = triton_add_shortcut  # resblock.py:157-175 (same arithmetic)

@@ -9,7 +9,8 @@ Backward (rms_norm.py:115-128): δμ_a = inv μ_γ δμ_z, δS_a = (inv μ_γ)²
 ``forward(ma, Sa, residual=(mr, Sr))`` adds a residual stream first and keeps the sum in
 ``stream``, in one pass (kernels/norm.py); ``backward(dmz, dSz, stream_delta=(dm, dS))``
 then adds the deltas that reached the stream behind the norm and returns the deltas of
-both addends. ``forward_int8`` gives the output in 8 bits for ``Int8Linear`` (no backward).
+both addends. The backward reads the stream, so what follows adds to a tensor of its own
+(``Add``, the next norm's ``residual``); after a change in place ``backward`` raises. ``forward_int8`` gives the output in 8 bits for ``Int8Linear`` (no backward).
 """
 
 from __future__ import annotations
@@ -24,6 +25,11 @@ from ..kernels.norm import (add_rmsnorm, add_rmsnorm_backward, add_rmsnorm_backw
                             add_rmsnorm_backward_update, add_rmsnorm_int8)
 from ..param_init import init_weight_bias_norm
 from ._params import contiguous_params
+
+
+def _version(t: Tensor) -> int:
+    """How often ``t`` (or what it is a view of) was changed in place."""
+    return 0 if t.is_inference() else t._version
 
 
 class RMSNorm(LearnableLayer):
@@ -75,6 +81,7 @@ class RMSNorm(LearnableLayer):
             hm, hS, mz, Sz, inv = add_rmsnorm(*self._rows_of(ma, Sa, *residual), self.mw, self.Sw,
                                               float(self.eps))
             self.ma_in, self.inv_rms = hm.view(-1, self.ni), inv.view(-1, 1)
+            self._stream_version = _version(self.ma_in)
             hm, hS, mz, Sz = self._shaped(ma.shape, hm, hS, mz, Sz)
             self.stream = (hm, hS)
             return mz, Sz
@@ -103,6 +110,9 @@ class RMSNorm(LearnableLayer):
         return q
 
     def _fused_backward(self, dmz, dSz, delta) -> tuple[Tensor, Tensor]:
+        if _version(self.ma_in) != self._stream_version:
+            raise RuntimeError("RMSNorm.backward: the residual stream was changed in place after "
+                               "the forward pass; add to a tensor of its own")
         mode, shape = self._param_mode, dmz.shape
         dmz, dSz, rm, rS = self._rows_of(dmz, dSz, *((None, None) if delta is None else delta))
         head = (dmz, dSz, self.ma_in, self.inv_rms)
