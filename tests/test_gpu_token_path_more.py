@@ -186,3 +186,20 @@ def test_the_square_of_a_scale_is_rounded_once(root):
         g_m, g_S = embedding_grad(ids[:k], dm[:k], dS[:k], V, scale=scale)
         assert torch.equal(g_m, t_m * scale)
         assert torch.equal(g_S, t_S * (scale * scale))
+
+
+# -- refusals -------------------------------------------------------------------------------
+
+
+def test_a_stream_of_other_rows_is_refused():
+    """As many values in another shape are not the stream of these deltas."""
+    from triton_tagi.kernels import add_rmsnorm_backward
+
+    g = gen(50)
+    dm, dS, h, inv, w = randn(g, 6, 4), -rand(g, 6, 4), randn(g, 6, 4), rand(g, 6), rand(g, 4)
+    ref = add_rmsnorm_backward(dm, dS, h, inv, w, w)
+    got = add_rmsnorm_backward(dm.view(2, 3, 4), dS.view(2, 3, 4), h, inv.view(2, 3), w, w)
+    assert all(torch.equal(a.view(b.shape), b) for a, b in zip(got, ref))
+    for other in (h.t().contiguous(), h.view(-1), h.view(3, 8)):
+        with pytest.raises(ValueError, match="do not match"):
+            add_rmsnorm_backward(dm, dS, other, inv, w, w)

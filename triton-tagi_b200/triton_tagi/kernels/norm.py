@@ -86,7 +86,7 @@ def _backward(mode, dmz, dSz, hm, inv, mw, Sw, rm, rS, sums=None, d_mw=None, d_S
     _pair(name, rm, rS)
     dev, rows, width = _rows(name, mw, Sw, dmz, dSz, rm, rS)
     check_f32(dmz, hm, inv)
-    if hm.numel() != rows * width or inv.numel() != rows:
+    if hm.numel() != rows * width or hm.shape[-1:] != (width,) or inv.numel() != rows:
         raise ValueError(f"{name}: the stream {tuple(hm.shape)} and 1/rms {tuple(inv.shape)} do "
                          f"not match {rows} rows of {width}")
     dmz, dSz, hm, inv, rm, rS = _cont(dmz, dSz, hm, inv, rm, rS)
