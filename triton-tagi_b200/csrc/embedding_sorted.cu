@@ -146,9 +146,9 @@ struct SortArgs {
 // longer ones are read and ranked again.
 //
 // Bound by latency: 9 us of a pass are four barriers, the remote counts and scattered
-// 8-byte stores, which the SMs of the cluster issue one sector per clock (16 CTAs beat 8:
-// 28 us against 41 for two passes over 65001 tokens; 512 threads beat 1024, whose
-// registers spill: 22 us). 16384 ids below 64, one pass: 8 us.
+// 8-byte stores, which the SMs of the cluster issue one sector per clock. Two passes over
+// 65001 tokens: 20 us; one over 16384 ids below 64: 8 us. An earlier version of it decided
+// for 16 CTAs (28 us against 41 with 8); 512 threads, as the registers of 1024 spill.
 template <int IDT>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a) {
     __shared__ int count[kSortWarps][kBins];

@@ -615,8 +615,8 @@ __global__ void __launch_bounds__(256) back_finish_kernel(const double* part, in
     if (lane == 0 && j < ni) gamma_out(out, j, ni, a, b);
 }
 
-// Threads along the columns of `vecs` vectors, and slices of rows: three blocks per SM
-// (what their registers allow), 2 rows or more for each of a block's groups.
+// Threads along the columns of `vecs` vectors, and slices of rows: two blocks per SM (what
+// the registers allow: 512 threads of 64), 2 rows or more for each of a block's groups.
 int back_x(int64_t vecs) {
     int x = 32;
     while (x < kBackCols && x < vecs) x *= 2;
